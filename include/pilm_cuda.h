@@ -469,6 +469,67 @@ int ekernel_paged_attention_verify_f32(const ekernel_paged_attn_desc_t *desc, co
 /* out = silu(gate) * up in fp32 (layers.py:193); gate_up is [rows, 2*inter]. */
 int ekernel_silu_mul_f32(const float *gate_up, size_t rows, size_t inter, float *out);
 
+/* ---- 8-bit KV cache: e4m3 codes with one scale per page and KV head.  The reference caches
+ * in the model's dtype (physical_kv.py:30-33) and has no counterpart to these calls.
+ *
+ * Layout: k_cache and v_cache [num_blocks, 16, n_kv, 128] e4m3 codes (bytes), k_scale and
+ * v_scale [num_blocks, n_kv] fp32; an element is code * scale.  Half the bytes of the bf16
+ * cache plus 1/512, so attention over long contexts, which is bound by reading the cache,
+ * takes about half the time.  Page ids, slots and block tables mean what they do for the
+ * bf16 cache.  Both caches 16-byte aligned; scales finite and not negative. ---- */
+
+/* ekernel_qk_norm_rope_kv_append into an 8-bit cache.  Computed in fp32 with one rounding per
+ * output (q to bf16, K and V to e4m3).
+ *  - A page's new scale is 2^e, e the least integer with amax <= 448 * 2^e, amax being the
+ *    largest magnitude among the rows written now and the tokens kept (0 gives e = 0).  Kept
+ *    are the tokens at offsets below the first offset written: their codes are rounded to the
+ *    new scale.  Tokens above (rejected drafts, an earlier owner's) are stale and count for
+ *    nothing, so a row at offset 0 starts its page anew.
+ *  - The rows of one page must follow one another in row order (a sequence's rows do); rows
+ *    with a slot outside [0, num_blocks * 16) are not written and may stand anywhere.  Where
+ *    rows repeat a slot the last one stands.
+ *  - NaN is stored as 0; an infinity saturates at the largest code of the page's scale, which
+ *    the finite values set.  The codes 0x7F and 0xFF (NaN) are never written.
+ *  - Positions outside [0, rope_rows) are not rotated. */
+int ekernel_qk_norm_rope_kv_append_kv8(const ekernel_paged_attn_desc_t *desc, const uint16_t *qkv,
+                                       const uint16_t *q_norm_w, const uint16_t *k_norm_w, const float *rope_cos,
+                                       const float *rope_sin, const int32_t *positions, const int32_t *slot_mapping,
+                                       uint8_t *k_cache, uint8_t *v_cache, float *k_scale, float *v_scale,
+                                       uint16_t *q_out, uint16_t *gate_out);
+
+/* The same with the projection given as the split-K partial sums of a deferred W4 linear
+ * ([splits][total_q][qkv_stride] fp32): the results are those of the summed projection. */
+int ekernel_qk_norm_rope_kv_append_kv8_splitk(const ekernel_paged_attn_desc_t *desc, const float *partials,
+                                              int32_t splits, const uint16_t *q_norm_w, const uint16_t *k_norm_w,
+                                              const float *rope_cos, const float *rope_sin, const int32_t *positions,
+                                              const int32_t *slot_mapping, uint8_t *k_cache, uint8_t *v_cache,
+                                              float *k_scale, float *v_scale, uint16_t *q_out, uint16_t *gate_out);
+
+/* Paged attention over an 8-bit cache: ekernel_paged_attention_verify's arguments and masks,
+ * and any row count per sequence from one token to a prompt chunk.
+ *  - window > 0: the row at position p sees the keys in (p - window, p] and the first `sinks`
+ *    keys (never beyond p); pages outside are not read.  window = 0: every key <= p, and sinks
+ *    is ignored.
+ *  - Rows whose position is negative (a context shorter than the rows) see no key: their
+ *    output is 0.  Rows of `out` from cu_q[num_seqs] on are not written.
+ *  - A block id outside [0, num_blocks) reads as a page of zeros.  Bytes past the context are
+ *    read as nothing whatever they hold; NaN codes (0x7F, 0xFF) below it must not occur.
+ *  - Scores, softmax and sums are fp32 (queries and keys multiply exactly); probabilities are
+ *    rounded to f16 for the product with V; the output is rounded once, after the gate.
+ *  - workspace: at least ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks)
+ *    bytes, 16-byte aligned, its contents undefined before and after.  The library allocates
+ *    none of its own, so calls that may overlap on the GPU (other streams, other graphs) need
+ *    only workspaces of their own.
+ *  - max_q_len and max_context must bound the batch's rows and contexts: they size the
+ *    workspace and the launch (a captured launch stays valid while the bounds hold). */
+size_t ekernel_paged_attention_kv8_workspace_bytes(const ekernel_paged_attn_desc_t *desc, size_t window,
+                                                   size_t sinks);
+int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, const uint16_t *q,
+                                       const uint8_t *k_cache, const uint8_t *v_cache, const float *k_scale,
+                                       const float *v_scale, const int32_t *block_table, const int32_t *cu_q,
+                                       const int32_t *context_lens, const uint16_t *gate, size_t window, size_t sinks,
+                                       void *workspace, size_t workspace_bytes, uint16_t *out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,10 @@ KERNEL_SYMBOLS = [
     "ekernel_qk_norm_rope_kv_append_f32",
     "ekernel_paged_attention_verify_f32",
     "ekernel_silu_mul_f32",
+    "ekernel_qk_norm_rope_kv_append_kv8",
+    "ekernel_qk_norm_rope_kv_append_kv8_splitk",
+    "ekernel_paged_attention_kv8_workspace_bytes",
+    "ekernel_paged_attention_verify_kv8",
 ]
 
 
@@ -224,6 +228,13 @@ def _configure(lib) -> None:
     lib.ekernel_qk_norm_rope_kv_append.argtypes = [ctypes.POINTER(PagedAttnDesc)] + [_vp] * 11
     lib.ekernel_paged_attention_verify.argtypes = [ctypes.POINTER(PagedAttnDesc)] + [_vp] * 8
     lib.ekernel_paged_attention_verify_noalloc.argtypes = [ctypes.POINTER(PagedAttnDesc)] + [_vp] * 8
+    lib.ekernel_qk_norm_rope_kv_append_kv8.argtypes = [ctypes.POINTER(PagedAttnDesc)] + [_vp] * 13
+    lib.ekernel_qk_norm_rope_kv_append_kv8_splitk.argtypes = ([ctypes.POINTER(PagedAttnDesc), _vp, _i32] +
+                                                              [_vp] * 12)
+    lib.ekernel_paged_attention_kv8_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnDesc), _sz, _sz]
+    lib.ekernel_paged_attention_kv8_workspace_bytes.restype = _sz
+    lib.ekernel_paged_attention_verify_kv8.argtypes = ([ctypes.POINTER(PagedAttnDesc)] + [_vp] * 9 +
+                                                       [_sz, _sz, _vp, _sz, _vp])
     lib.ekernel_argmax_top2_f32.argtypes = [ctypes.POINTER(AcceptDesc), _vp, _vp, _vp, _vp]
     lib.ekernel_argmax_top2_bf16.argtypes = [ctypes.POINTER(AcceptDesc), _vp, _vp, _vp, _vp]
     lib.ekernel_verify_accept_greedy.argtypes = [ctypes.POINTER(AcceptDesc)] + [_vp] * 7

@@ -18,7 +18,8 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libpilm_cuda.so"
 INCLUDE = HERE.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-SOURCES = ["runtime.cu", "linear.cu", "linear_tc.cu", "norm.cu", "attention.cu", "accept.cu", "mtp.cu", "f32.cu"]
+SOURCES = ["runtime.cu", "linear.cu", "linear_tc.cu", "norm.cu", "attention.cu", "accept.cu", "mtp.cu", "f32.cu",
+           "kv8_append.cu", "kv8_attention.cu"]
 
 
 def nvcc() -> str:

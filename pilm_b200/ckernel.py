@@ -380,6 +380,113 @@ def paged_attention_verify(desc, q, k_cache, v_cache, block_table, cu_q, context
            "ekernel_paged_attention_verify")
 
 
+# ---- 8-bit KV cache: e4m3 codes, one scale per page and KV head ----------------------------
+
+def _kv8(device: torch.device, *tensors) -> None:
+    """Checks of the 8-bit cache calls: (name, tensor, dtype, least number of elements) each, on
+    one CUDA device and contiguous, since the kernels go by raw pointers."""
+    for name, t, dtype, numel in tensors:
+        if t is None:
+            continue
+        if t.dtype != dtype or t.device != device or t.numel() < numel or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements on {device}, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}"
+                             + ("" if t.is_contiguous() else " (not contiguous)"))
+
+
+def _kv8_cache(desc, device, k_cache, v_cache, k_scale, v_scale) -> None:
+    if device.type != "cuda":
+        raise ValueError("the 8-bit cache calls take CUDA tensors")
+    n = desc.num_blocks * desc.n_kv_heads
+    codes = n * desc.block_size * desc.head_dim
+    _kv8(device, ("k_cache", k_cache, torch.uint8, codes), ("v_cache", v_cache, torch.uint8, codes),
+         ("k_scale", k_scale, torch.float32, n), ("v_scale", v_scale, torch.float32, n))
+
+
+def _on(device: torch.device):
+    """Launch on the tensors' device, whichever is current."""
+    return torch.cuda.device(device)
+
+
+def _append_kv8_args(desc, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache, k_scale,
+                     v_scale, q_out, gate_out):
+    dev, hd, t = k_cache.device, desc.head_dim, desc.total_q
+    _kv8_cache(desc, dev, k_cache, v_cache, k_scale, v_scale)
+    nf = desc.rope_rows * (desc.rot_dim // 2)
+    _kv8(dev, ("q_norm_w", q_norm_w, torch.bfloat16, hd), ("k_norm_w", k_norm_w, torch.bfloat16, hd),
+         ("rope_cos", rope_cos, torch.float32, nf), ("rope_sin", rope_sin, torch.float32, nf),
+         ("positions", positions, torch.int32, t), ("slot_mapping", slot_mapping, torch.int32, t),
+         ("q_out", q_out, torch.bfloat16, t * desc.n_heads * hd),
+         ("gate_out", gate_out, torch.bfloat16, t * desc.n_heads * hd if desc.output_gate else 0))
+    return (q_norm_w.data_ptr(), k_norm_w.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), positions.data_ptr(),
+            slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            q_out.data_ptr(), _p(gate_out))
+
+
+def qk_norm_rope_kv_append_kv8(desc, qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache,
+                               v_cache, k_scale, v_scale, q_out, gate_out=None) -> None:
+    """QK-RMSNorm + RoPE of the rows of qkv [total_q, qkv_stride], K and V quantized into their
+    pages of an 8-bit cache (uint8 e4m3 codes [num_blocks, 16, n_kv, 128], fp32 scales
+    [num_blocks, n_kv]; see include/pilm_cuda.h for the scale's rule).  Written: q_out, gate_out
+    when the descriptor is gated, the caches and scales."""
+    _kv8(k_cache.device, ("qkv", qkv, torch.bfloat16, desc.total_q * desc.qkv_stride))
+    args = _append_kv8_args(desc, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache,
+                            k_scale, v_scale, q_out, gate_out)
+    with _on(k_cache.device):
+        _stream()
+        _check(abi.lib().ekernel_qk_norm_rope_kv_append_kv8(desc, qkv.data_ptr(), *args),
+               "ekernel_qk_norm_rope_kv_append_kv8")
+
+
+def qk_norm_rope_kv_append_kv8_splitk(desc, partials, splits, q_norm_w, k_norm_w, rope_cos, rope_sin, positions,
+                                      slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out, gate_out=None) -> None:
+    """qk_norm_rope_kv_append_kv8 with the projection given as a deferred W4 linear's split-K
+    partial sums ([splits, total_q, qkv_stride] fp32)."""
+    _kv8(k_cache.device, ("partials", partials, torch.float32, splits * desc.total_q * desc.qkv_stride))
+    args = _append_kv8_args(desc, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache,
+                            k_scale, v_scale, q_out, gate_out)
+    with _on(k_cache.device):
+        _stream()
+        _check(abi.lib().ekernel_qk_norm_rope_kv_append_kv8_splitk(desc, partials.data_ptr(), int(splits), *args),
+               "ekernel_qk_norm_rope_kv_append_kv8_splitk")
+
+
+def _window(window: int, sinks: int) -> None:
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+
+
+def paged_attention_kv8_workspace_bytes(desc, window: int = 0, sinks: int = 0) -> int:
+    """Bytes of workspace that paged_attention_verify_kv8 needs for this descriptor."""
+    _window(window, sinks)
+    return int(abi.lib().ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks))
+
+
+def paged_attention_verify_kv8(desc, q, k_cache, v_cache, k_scale, v_scale, block_table, cu_q, context_lens, gate, out,
+                               window: int = 0, sinks: int = 0, workspace: Optional[torch.Tensor] = None) -> None:
+    """Causal attention of each sequence's last rows over its pages of an 8-bit cache; with
+    window > 0 a row at position p sees the keys in (p - window, p] and the first `sinks`.
+    workspace: a uint8 tensor of paged_attention_kv8_workspace_bytes; allocated here when None.
+    Calls that may run at the same time need workspaces of their own."""
+    _window(window, sinks)
+    dev, rows = k_cache.device, desc.total_q * desc.n_heads * desc.head_dim
+    _kv8_cache(desc, dev, k_cache, v_cache, k_scale, v_scale)
+    _kv8(dev, ("q", q, torch.bfloat16, rows), ("out", out, torch.bfloat16, rows),
+         ("gate", gate, torch.bfloat16, rows if desc.output_gate else 0),
+         ("block_table", block_table, torch.int32, desc.num_seqs * desc.max_blocks_per_seq),
+         ("cu_q", cu_q, torch.int32, desc.num_seqs + 1), ("context_lens", context_lens, torch.int32, desc.num_seqs),
+         ("workspace", workspace, torch.uint8, 0))
+    with _on(dev):
+        _stream()
+        if workspace is None:
+            workspace = torch.empty(paged_attention_kv8_workspace_bytes(desc, window, sinks), dtype=torch.uint8,
+                                    device=dev)
+        _check(abi.lib().ekernel_paged_attention_verify_kv8(
+            desc, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            block_table.data_ptr(), cu_q.data_ptr(), context_lens.data_ptr(), _p(gate), window, sinks,
+            workspace.data_ptr(), workspace.numel(), out.data_ptr()), "ekernel_paged_attention_verify_kv8")
+
+
 # ---- fp32-activation path (the W8A32 configuration) --------------------------------------
 
 def embedding_f32(ids: torch.Tensor, table: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -51,6 +51,9 @@ int linear_bf16(int qf, int gs, const void *A, int M, int K, const void *W, cons
                 const char *what, bool kpairs = false, float *defer = nullptr, size_t defer_cap = 0,
                 int *defer_splits = nullptr, unsigned long long *amax = nullptr, int *amax_done = nullptr);
 
+// Descriptor checks of the 8-bit KV cache entry points (kv8_append.cu).
+int kv8_check_desc(const ekernel_paged_attn_desc_t *d, const char *what);
+
 // cuTensorMapEncodeTiled, reached through the runtime's driver entry point (no link
 // against libcuda); null if the driver does not provide it.
 typedef CUresult (*TensorMapEncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
