@@ -2,77 +2,843 @@
 //
 // out = softmax(q k^T / sqrt(128)) v for rows at the end of each sequence's context; a row at
 // position p sees keys <= p, or with a window the keys in (p - window, p] and the first sinks.
+// With k = ks * K8 and v = vs * V8 of a page, codes K8 and V8 being f16 values exactly:
+//   s = (q . K8) * (ks / sqrt(128))      the scale of a page multiplies 16 scores, not 2048 codes
+//   o = sum_pages (vs / vref) * (p . V8) * vref / sum p,   vref the largest vs so far
+//
+// The reference's attention is FullAttention.forward (src/models/qwen3/attention.py:98-139);
+// it caches in the model's dtype, so there is no reference result to reproduce here: scores
+// stay in fp32.
 #include "fp8.cuh"
 
 using namespace pilm;
 
+// Set when a bounded wait gave up (read and cleared in synchronous mode).
+static __device__ int g_kv8_error;
+
 namespace {
 
 constexpr int kHD = kKv8HD;
+constexpr uint32_t kWaitLimit = 1u << 22;  // polls before a wait gives up
 
-struct AttnParams {
-    const __nv_bfloat16 *q, *gate;
-    const uint8_t *kc, *vc;
-    const float *ks, *vs;
-    const int32_t *block_table, *cu_q, *ctx;
-    __nv_bfloat16 *out;
-    int nh, nkv, num_seqs, max_blocks, num_blocks;
-    long long window, sinks;
-    float scale;
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t *b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t *b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait; false once the limit is reached or another warp gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+        if (mbar_try_wait(b, parity)) return true;
+        if ((i & 255) == 255 && *abort_flag) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            dst),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+// The barrier's phase also waits for this thread's cp.async so far (one of its expected arrivals).
+__device__ __forceinline__ void cp_async_arrive(uint64_t *b) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
+// Probabilities are held as 2^14 exp(s - max), so that their f16 rounding keeps 11 bits down to
+// 2^-28 of the largest and drops nothing above 2^-39: a long tail of small ones still counts.
+constexpr float kProbBits = 14.f;
+
+// ---------------------------------------------------------------------------------
+// Geometry shared by the kernels.  A batch's rows are cut into groups: group (b, rg) holds the
+// rows rho in [rg * rpg, (rg + 1) * rpg) of sequence b, rho = j * gsz + g for query row j and
+// head g of a KV head's group.  A group's keys are a list of nv pages: the first n_sink pages
+// of the sequence, then those from lo_page on.
+// ---------------------------------------------------------------------------------
+struct Geometry {
+    const int32_t *cu_q, *ctx;
+    int gsz, rpg, rgs;  // query heads per KV head, rows per group, groups per sequence
+    int window, sinks;  // window 0: none
+};
+struct Group {
+    int q0, rows, p0, ctx;      // first row, rows (rho) of the sequence, position of row j = 0
+    int rho0, rho1;             // this group's rows
+    int n_sink, lo_page, nv;
 };
 
-// One warp per (row, head), 4 dims per lane, one key at a time: online softmax in fp32.
-__global__ void kv8_attn_simple(const AttnParams p, int total_q) {
-    pdl_entry();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int row = (int)(item / p.nh), h = (int)(item % p.nh);
-    if (row >= total_q || row >= p.cu_q[p.num_seqs]) return;
-    int lo = 0, hi = p.num_seqs - 1;
-    while (lo < hi) {  // the last sequence that starts at or before the row
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.cu_q[mid] <= row) lo = mid; else hi = mid - 1;
+__device__ __forceinline__ Group group_of(const Geometry &g, int vs) {
+    Group r;
+    const int b = vs / g.rgs, rg = vs % g.rgs;
+    r.q0 = g.cu_q[b];
+    const int q_len = g.cu_q[b + 1] - r.q0;
+    r.ctx = g.ctx[b];
+    r.rows = q_len * g.gsz;
+    r.p0 = r.ctx - q_len;
+    r.rho0 = rg * g.rpg;
+    r.rho1 = min(r.rows, r.rho0 + g.rpg);
+    r.n_sink = r.lo_page = r.nv = 0;
+    if (r.rho0 >= r.rho1) return r;
+    const int pmin = r.p0 + r.rho0 / g.gsz, pmax = r.p0 + (r.rho1 - 1) / g.gsz;
+    if (pmax < 0) return r;
+    const int end = (pmax >> 4) + 1;
+    if (g.window > 0) {
+        r.lo_page = pmin - g.window + 1 > 0 ? (pmin - g.window + 1) >> 4 : 0;
+        r.n_sink = min((g.sinks + 15) >> 4, r.lo_page);
     }
-    const int b = lo, kvh = h / (p.nh / p.nkv);
-    const int q_end = p.cu_q[b + 1], ctx = p.ctx[b];
-    if (row >= q_end) return;
-    const int pos = ctx - (q_end - row);
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-    const size_t base = ((size_t)row * p.nh + h) * kHD + 4 * lane;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q[j] = bf2f(p.q[base + j]) * p.scale;
-    const long long first = p.window > 0 ? (long long)pos - p.window + 1 : 0;
-    for (int key = 0; key <= pos; ++key) {
-        if (key < first && key >= p.sinks) {
-            key = (int)first - 1;
-            continue;
+    r.nv = r.n_sink + end - r.lo_page;
+    return r;
+}
+__device__ __forceinline__ int page_of(const Group &g, int v) { return v < g.n_sink ? v : v - g.n_sink + g.lo_page; }
+
+// CTA whose range [c*T/G, (c+1)*T/G) holds unit x
+__device__ __forceinline__ int cta_of(long long x, long long T, int G) {
+    int c = (int)((x * G) / T);
+    if (c >= G) c = G - 1;
+    while (c + 1 < G && ((long long)(c + 1) * T) / G <= x) ++c;
+    while (c > 0 && ((long long)c * T) / G > x) --c;
+    return c;
+}
+
+// ---------------------------------------------------------------------------------
+// Token kernel: decode and verify rows, bound by reading the cache.
+//
+// One CTA per SM.  The groups' pages, in blocks of `pps`, form one list that the CTAs of a head
+// group share evenly: a producer warp streams whole blocks (K and V of `hg` KV heads) through a
+// TMA ring, and consumer warp (h, c, k) takes head h, row tile c (16 rows) and pages 2k, 2k + 1
+// of each block, so every byte is read from HBM once and 8 warps share the conversions.
+//
+// Per pair of pages a warp computes S = Q K8^T and O += P V8 with mma.sync m16n8k16 on f16: the
+// codes are converted in registers as they leave shared memory (two per instruction).  Both
+// products sum over an index whose order is free, and each order is chosen so that a thread's
+// operand is contiguous in the cache as it lies there: thread (g, c) = (lane / 4, lane % 4) holds
+// dims 32c .. 32c + 31 of a key for S, and dims 16g .. 16g + 15 of its four keys for O, where
+// four byte permutes pair the keys.  With the TMA's 128-byte swizzle all these 16-byte
+// shared-memory loads are free of bank conflicts.
+//
+// The tcgen05 pipe does not fit these shapes: one token's rows (gsz = 4, say) would fill 4 of its
+// 128 rows.  mma.sync at 16 rows keeps up with HBM.
+// ---------------------------------------------------------------------------------
+constexpr int kTokWarps = 8;      // consumer warps at most
+constexpr int kTokGroups = 4096;  // groups per launch (their prefix is kept in shared memory)
+constexpr int kTokStages = 8;     // ring stages at most
+constexpr int kRec = kHD + 4;     // a partial: O[128] normalised, max (base 2), sum, two pad floats
+
+struct TokParams {
+    Geometry geo;
+    const __nv_bfloat16 *q, *gate;
+    const float *ks, *vs;
+    const int32_t *block_table;
+    __nv_bfloat16 *out;
+    float *part;      // [head groups][G][2][hg * rpg][kRec]
+    int *prefix_out;  // [groups + 1]: blocks before each group, for the merge
+    int nh, nkv, max_blocks, num_blocks;
+    int groups, hg, ch, kw, pps, stages, G;
+};
+
+// Rows of a group that sees no key.
+__device__ void zero_rows(const TokParams &p, const Group &g, int head0, int heads) {
+    for (int i = threadIdx.x; i < (g.rho1 - g.rho0) * heads * (kHD / 8); i += blockDim.x) {
+        const int d = i % (kHD / 8), h = i / (kHD / 8) % heads, rho = g.rho0 + i / (kHD / 8) / heads;
+        if (head0 + h >= p.nkv) continue;
+        const size_t row = (size_t)(g.q0 + rho / p.geo.gsz) * p.nh + (head0 + h) * p.geo.gsz + rho % p.geo.gsz;
+        *reinterpret_cast<uint4 *>(p.out + row * kHD + 8 * d) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+__global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const __grid_constant__ CUtensorMap kmap,
+                                                                           const __grid_constant__ CUtensorMap vmap,
+                                                                           const TokParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int s_prefix[kTokGroups + 1];
+    __shared__ __align__(8) uint64_t full_bar[kTokStages], empty_bar[kTokStages], meet_bar;
+    __shared__ float s_scale[kTokStages][2][16];  // [stage][K, V][page of the block * hg + head]
+    __shared__ uint32_t s_valid[kTokStages];      // bit i: page i of the block has a valid id
+    __shared__ int s_abort;
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int consumers = p.hg * p.ch * p.kw;
+    const int cta = blockIdx.x, head0 = blockIdx.y * p.hg;
+    const uint32_t page_bytes = (uint32_t)p.hg * 2048;        // K (or V) of one page, hg heads
+    const uint32_t stage_bytes = 2 * page_bytes * p.pps;      // K pages, then V pages
+    if (threadIdx.x == 0) {
+        for (int st = 0; st < p.stages; ++st) {
+            mbar_init(&full_bar[st], 1 + 32);
+            mbar_init(&empty_bar[st], (uint32_t)consumers);
         }
-        const int blk = (key >> 4) < p.max_blocks ? p.block_table[(size_t)b * p.max_blocks + (key >> 4)] : -1;
-        const bool ok = blk >= 0 && blk < p.num_blocks;
-        float s = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (ok) {
-            const size_t at = (((size_t)blk * kKv8Page + (key & 15)) * p.nkv + kvh) * kHD + 4 * lane;
-            const float ks = p.ks[(size_t)blk * p.nkv + kvh], vs = p.vs[(size_t)blk * p.nkv + kvh];
-            const uint32_t kw = *reinterpret_cast<const uint32_t *>(p.kc + at);
-            const uint32_t vw = *reinterpret_cast<const uint32_t *>(p.vc + at);
-            const float2 k0 = f16x2_to_f32x2(e4m3x2_to_f16x2(kw)), k1 = f16x2_to_f32x2(e4m3x2hi_to_f16x2(kw));
-            const float2 v0 = f16x2_to_f32x2(e4m3x2_to_f16x2(vw)), v1 = f16x2_to_f32x2(e4m3x2hi_to_f16x2(vw));
-            s = (q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y) * ks;
-            v[0] = v0.x * vs, v[1] = v0.y * vs, v[2] = v1.x * vs, v[3] = v1.y * vs;
+        mbar_init(&meet_bar, (uint32_t)consumers);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_wait();
+    if (warp == 0) {  // blocks before each group
+        int carry = 0;
+        if (lane == 0) s_prefix[0] = 0;
+        for (int v0 = 0; v0 < p.groups; v0 += 32) {
+            const int v = v0 + lane;
+            int n = v < p.groups ? (group_of(p.geo, v).nv + p.pps - 1) / p.pps : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, n, o);
+                if (lane >= o) n += up;
+            }
+            if (v < p.groups) s_prefix[v + 1] = carry + n;
+            carry += __shfl_sync(0xffffffffu, n, 31);
         }
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), a = __expf(m - mn), pr = __expf(s - mn);
-        m = mn;
-        l = l * a + pr;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = o[j] * a + pr * v[j];
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float r = l > 0.f ? o[j] / l : 0.f;
-        if (p.gate) r = r / (1.f + __expf(-bf2f(p.gate[base + j])));
-        p.out[base + j] = f2bf(r);
+    __syncthreads();
+    if (cta == 0 && blockIdx.y == 0 && p.prefix_out)
+        for (int v = threadIdx.x; v <= p.groups; v += blockDim.x) p.prefix_out[v] = s_prefix[v];
+    for (int v = cta; v < p.groups; v += p.G)
+        if (s_prefix[v] == s_prefix[v + 1]) zero_rows(p, group_of(p.geo, v), head0, p.hg);
+    const long long T = s_prefix[p.groups];
+    const long long x0 = ((long long)cta * T) / p.G, x1 = ((long long)(cta + 1) * T) / p.G;
+    if (x0 >= x1) return;
+    int v_first;  // the group of block x0
+    {
+        int lo = 0, hi = p.groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
+        }
+        v_first = lo;
     }
+    const uint32_t ring = smem_u32(smem);
+
+    if (warp == consumers) {
+        // ---- producer ----
+        int v = v_first, issued = 0;
+        Group g = group_of(p.geo, v);
+        bool ok = true;
+        // a block's page ids are fetched one block ahead (lane i: page i of the block)
+        auto fetch = [&](long long x, int &vv, Group &gg) {
+            if (x >= x1) return -1;
+            while (x >= s_prefix[vv + 1]) gg = group_of(p.geo, ++vv);
+            const int vp = (int)(x - s_prefix[vv]) * p.pps + lane;
+            int blk = -1;
+            if (lane < p.pps && vp < gg.nv) {
+                const int pg = page_of(gg, vp);
+                if (pg < p.max_blocks) blk = p.block_table[(size_t)(vv / p.geo.rgs) * p.max_blocks + pg];
+                if (blk < 0 || blk >= p.num_blocks) blk = -1;
+            }
+            return blk;
+        };
+        int next = fetch(x0, v, g);
+        for (long long x = x0; x < x1; ++x, ++issued) {
+            const int blk = next;
+            next = fetch(x + 1, v, g);
+            const int st = issued % p.stages;
+            if (issued >= p.stages)
+                ok = mbar_wait(&empty_bar[st], (uint32_t)(issued / p.stages - 1) & 1u, &s_abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const uint32_t valid = __ballot_sync(0xffffffffu, blk >= 0);
+            if (lane == 0) {
+                s_valid[st] = valid;  // published by the arrive
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_expect_tx(&full_bar[st], (uint32_t)__popc(valid) * 2 * page_bytes);
+            }
+            __syncwarp();
+            if (blk >= 0) {
+                const uint32_t dst = ring + st * stage_bytes + lane * page_bytes;
+                tma_load_3d(dst, &kmap, &full_bar[st], 0, blk * kKv8Page, head0);
+                tma_load_3d(dst + p.pps * page_bytes, &vmap, &full_bar[st], 0, blk * kKv8Page, head0);
+            }
+            const int pg = lane / p.hg, h = lane % p.hg;  // pps * hg <= 16 scales of each kind
+            const int src = __shfl_sync(0xffffffffu, blk, pg & 31);
+            if (pg < p.pps && src >= 0 && head0 + h < p.nkv) {
+                const size_t at = (size_t)src * p.nkv + head0 + h;
+                cp_async_4(smem_u32(&s_scale[st][0][lane]), p.ks + at);
+                cp_async_4(smem_u32(&s_scale[st][1][lane]), p.vs + at);
+            }
+            cp_async_arrive(&full_bar[st]);
+        }
+        if (!__all_sync(0xffffffffu, ok) && lane == 0) {
+            s_abort = 1;
+            atomicExch(&g_kv8_error, 1);
+        }
+        // every copy issued lands before the CTA may exit
+        for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&full_bar[j % p.stages], (uint32_t)(j / p.stages) & 1u);
+                 ++i) {
+            }
+        return;
+    }
+    if (warp > consumers) return;
+
+    // ---- consumer warp (h, c, k) ----
+    const int k_of = warp % p.kw, c_of = warp / p.kw % p.ch, h_of = warp / (p.kw * p.ch);
+    const int g4 = lane >> 2, c4 = lane & 3;
+    const int head = head0 + h_of;
+    const bool head_ok = head < p.nkv;
+    // byte offsets of this thread's loads in one head's 2 KB tile (rows of 128 B, 16-byte chunk i
+    // of row r at i ^ (r & 7))
+    uint32_t k_off[2][2], v_off[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) k_off[t][i] = (8 * t + g4) * 128 + (((2 * c4 + i) ^ g4) << 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 2 * c4 + (i & 1) + 8 * (i >> 1);
+        v_off[i] = row * 128 + ((g4 ^ (row & 7)) << 4);
+    }
+    // all consumer warps meet (bounded, unlike a hardware barrier whose partner has given up)
+    int met = 0;
+    auto meet = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&meet_bar);
+        const bool w = __all_sync(0xffffffffu, mbar_wait(&meet_bar, (uint32_t)met++ & 1u, &s_abort));
+        if (!w && lane == 0) {
+            s_abort = 1;
+            atomicExch(&g_kv8_error, 1);
+        }
+        return w;
+    };
+    int done = 0;  // blocks consumed
+    int v = v_first;
+    bool ok = true;
+    for (long long x = x0; x < x1 && ok;) {
+        while (x >= s_prefix[v + 1]) ++v;
+        const Group g = group_of(p.geo, v);
+        const long long seg1 = min(x1, (long long)s_prefix[v + 1]);
+        const bool whole = x == s_prefix[v] && seg1 == s_prefix[v + 1];
+        const int slot = x == x0 ? 0 : 1;
+        const int tile0 = g.rho0 + 16 * c_of;
+        const bool active = head_ok && tile0 < g.rho1;
+        const int tile1 = min(g.rho1, tile0 + 16);
+
+        // queries: row r in f16 as q * 2^k, the largest magnitude in [2^14, 2^15).  Exact for bf16
+        // elements down to 2^-29 of the largest; 2^-k goes into the row's score factor.
+        uint32_t qf[8][4];
+        float rowf[2];
+        int qpos[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const int rho = tile0 + g4 + 8 * hh;
+            const bool in = active && rho < tile1;
+            qpos[hh] = in ? g.p0 + rho / p.geo.gsz : -1;
+            float e[32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (in)
+                    w = *reinterpret_cast<const uint4 *>(
+                        p.q + ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD +
+                        32 * c4 + 8 * i);
+                const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    e[8 * i + 2 * j] = __uint_as_float(wd[j] << 16);
+                    e[8 * i + 2 * j + 1] = __uint_as_float(wd[j] & 0xffff0000u);
+                }
+            }
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(e[i]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            int sh = 14 - ((int)(__float_as_uint(mx) >> 23) - 127);
+            sh = sh > 126 ? 126 : sh;
+            const float up = pow2f(sh);
+            rowf[hh] = pow2f(-sh) * kScoreScale;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                qf[s][hh] = pack_f16(e[4 * s] * up, e[4 * s + 1] * up);
+                qf[s][2 + hh] = pack_f16(e[4 * s + 2] * up, e[4 * s + 3] * up);
+            }
+        }
+        // positions of the tile's first and last rows: pages every row sees whole need no mask
+        const int pmin = g.p0 + tile0 / p.geo.gsz, pmax = g.p0 + (tile1 - 1) / p.geo.gsz;
+
+        float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f, inv_vref = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+
+        for (; x < seg1; ++x, ++done) {
+            const int st = done % p.stages;
+            ok = mbar_wait(&full_bar[st], (uint32_t)(done / p.stages) & 1u, &s_abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) {
+                    s_abort = 1;
+                    atomicExch(&g_kv8_error, 1);
+                }
+                ok = false;
+                break;
+            }
+            const int vp = (int)(x - s_prefix[v]) * p.pps + 2 * k_of;
+            if (active && vp < g.nv) {
+                const uint32_t kb = ring + st * stage_bytes + (2 * k_of) * page_bytes + h_of * 2048;
+                const uint32_t vb = kb + p.pps * page_bytes;
+                const uint32_t valid = s_valid[st] >> (2 * k_of);
+                float kf[2], vf[2];
+                int key0[2];
+                bool masked = vp + 1 >= g.nv || (valid & 3u) != 3u;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = (2 * k_of + i) * p.hg + h_of;
+                    kf[i] = s_scale[st][0][at];
+                    vf[i] = s_scale[st][1][at];
+                    if (!((valid >> i) & 1u)) kf[i] = vf[i] = 0.f;
+                    key0[i] = page_of(g, vp + i) * 16;
+                    masked |= key0[i] + 15 > pmin ||
+                              (p.geo.window > 0 && key0[i] <= pmax - p.geo.window && key0[i] + 15 >= p.geo.sinks);
+                }
+                // ---- S = Q K8^T: two pages of two 8-key tiles, four independent chains ----
+                float s[2][2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t w[2][8];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const uint4 r = lds128(kb + i * page_bytes + k_off[t][hf]);
+                            w[t][4 * hf] = r.x, w[t][4 * hf + 1] = r.y, w[t][4 * hf + 2] = r.z, w[t][4 * hf + 3] = r.w;
+                        }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[i][t][j] = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            mma_f16(s[i][t], qf[k], e4m3x2_to_f16x2(w[t][k]), e4m3x2hi_to_f16x2(w[t][k]));
+                }
+                // ---- scores in base 2, masks, online softmax ----
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float &e = s[i][t][j];
+                            e *= rowf[j >> 1] * kf[i];
+                            if (masked) {
+                                const int key = key0[i] + 8 * t + 2 * c4 + (j & 1), qp = qpos[j >> 1];
+                                const bool see = vp + i < g.nv && key <= qp &&
+                                                 (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
+                                if (!((valid >> i) & 1u)) e = 0.f;  // a page of zeros
+                                if (!see) e = -INFINITY;
+                            }
+                            mx[j >> 1] = fmaxf(mx[j >> 1], e);
+                        }
+                const float vtop = fmaxf(vref, fmaxf(vf[0], vp + 1 < g.nv ? vf[1] : 0.f));
+                float fac[2], base[2];
+                bool moved = vtop != vref;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
+                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
+                    const float mn = fmaxf(m[hh], mx[hh]);
+                    moved |= mn != m[hh];
+                    const float mb = mn == -INFINITY ? 0.f : mn;
+                    fac[hh] = ex2(m[hh] - mb);
+                    base[hh] = kProbBits - mb;
+                    m[hh] = mn;
+                }
+                if (__any_sync(0xffffffffu, moved)) {  // a running maximum, or the V scale's, rose
+                    l[0] *= fac[0], l[1] *= fac[1];
+                    if (vtop != vref) {
+                        const float f = vref * (vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f);
+                        fac[0] *= f, fac[1] *= f;
+                        vref = vtop;
+                        inv_vref = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) {
+                        o[n][0] *= fac[0], o[n][1] *= fac[0];
+                        o[n][2] *= fac[1], o[n][3] *= fac[1];
+                    }
+                }
+                uint32_t pa[2][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float r = vf[i] * inv_vref;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            s[i][t][j] = ex2(s[i][t][j] + base[j >> 1]);
+                            l[j >> 1] += s[i][t][j];
+                        }
+                        pa[i][2 * t] = pack_f16(s[i][t][0] * r, s[i][t][1] * r);
+                        pa[i][2 * t + 1] = pack_f16(s[i][t][2] * r, s[i][t][3] * r);
+                    }
+                }
+                // ---- O += P V8 ----
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = lds128(vb + i * page_bytes + v_off[k]);
+                    if (masked) {  // bytes of keys that no row sees may be NaN codes: P = 0 there
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (key0[i] + 2 * c4 + (k & 1) + 8 * (k >> 1) > pmax || !((valid >> i) & 1u))
+                                w[k] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, b[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+                    const uint32_t c[4] = {w[2].x, w[2].y, w[2].z, w[2].w}, d[4] = {w[3].x, w[3].y, w[3].z, w[3].w};
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const uint32_t ab0 = __byte_perm(a[n], b[n], 0x5140), ab1 = __byte_perm(a[n], b[n], 0x7362);
+                        const uint32_t cd0 = __byte_perm(c[n], d[n], 0x5140), cd1 = __byte_perm(c[n], d[n], 0x7362);
+                        mma_f16(o[4 * n], pa[i], e4m3x2_to_f16x2(ab0), e4m3x2_to_f16x2(cd0));
+                        mma_f16(o[4 * n + 1], pa[i], e4m3x2hi_to_f16x2(ab0), e4m3x2hi_to_f16x2(cd0));
+                        mma_f16(o[4 * n + 2], pa[i], e4m3x2_to_f16x2(ab1), e4m3x2_to_f16x2(cd1));
+                        mma_f16(o[4 * n + 3], pa[i], e4m3x2hi_to_f16x2(ab1), e4m3x2hi_to_f16x2(cd1));
+                    }
+                }
+            }
+            // the segment's last stage stays held: the warps that share its rows meet there
+            if (x + 1 < seg1 || p.kw == 1) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_bar[st]);
+            }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
+            l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
+            // O in its own units: a convex combination of the values
+            const float f = l[hh] > 0.f ? __fdiv_rn(vref, l[hh]) : 0.f;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) o[n][2 * hh] *= f, o[n][2 * hh + 1] *= f;
+        }
+        if (p.kw > 1) {
+            // The kw warps of each (head, tile) hold different pages' shares: warps 1.. hand theirs
+            // to warp 0, which adds them in order.  With one row tile the last stage's memory has
+            // room for all of them at once; else they go one by one through a buffer of their own.
+            const int st = (done - 1) % p.stages;
+            const int at_once = p.ch == 1 ? p.kw - 1 : 1;
+            float *buf = reinterpret_cast<float *>(smem + (p.ch == 1 ? (size_t)st * stage_bytes
+                                                                     : (size_t)p.stages * stage_bytes)) +
+                         (size_t)(h_of * p.ch + c_of) * at_once * 16 * kRec;
+            ok = meet();  // every warp has read the stage
+            float w0[2] = {l[0], l[1]}, M[2] = {m[0], m[1]};
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int n = 0; n < 16; ++n) o[n][2 * hh] *= w0[hh], o[n][2 * hh + 1] *= w0[hh];
+            for (int k0 = 1; k0 < p.kw && ok; k0 += at_once) {
+                if (k_of >= k0 && k_of < k0 + at_once) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        float *row = buf + (k_of - k0) * 16 * kRec + (g4 + 8 * hh) * kRec;
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) {
+                            row[32 * c4 + n] = o[n][2 * hh];
+                            row[32 * c4 + 16 + n] = o[n][2 * hh + 1];
+                        }
+                        if (c4 == 0) row[kHD] = m[hh], row[kHD + 1] = l[hh];
+                    }
+                }
+                ok = meet();
+                if (k_of == 0 && ok) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        for (int k = 0; k < min(at_once, p.kw - k0); ++k) {
+                            const float *row = buf + k * 16 * kRec + (g4 + 8 * hh) * kRec;
+                            const float Mn = fmaxf(M[hh], row[kHD]), Mb = Mn == -INFINITY ? 0.f : Mn;
+                            const float f = ex2(M[hh] - Mb), w = ex2(row[kHD] - Mb);
+                            M[hh] = Mn;
+                            w0[hh] = w0[hh] * f + row[kHD + 1] * w;
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) {
+                                o[n][2 * hh] = o[n][2 * hh] * f + w * row[32 * c4 + n];
+                                o[n][2 * hh + 1] = o[n][2 * hh + 1] * f + w * row[32 * c4 + 16 + n];
+                            }
+                        }
+                }
+                if (at_once == 1) ok = meet() && ok;  // before the buffer's next use
+            }
+            if (!ok) break;
+            if (k_of == 0)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const float f = w0[hh] > 0.f ? __fdiv_rn(1.f, w0[hh]) : 0.f;
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) o[n][2 * hh] *= f, o[n][2 * hh + 1] *= f;
+                    m[hh] = M[hh], l[hh] = w0[hh];
+                }
+            // writes here come before the copies into this stage
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty_bar[st]);
+        }
+        if (!active || k_of > 0) continue;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const int rho = tile0 + g4 + 8 * hh;
+            if (rho >= tile1) continue;
+            if (whole) {
+                const size_t ob = ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const size_t at = ob + 32 * c4 + 16 * half + 8 * i;
+                        float e[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) e[j] = o[8 * i + j][2 * hh + half];
+                        if (p.gate) {
+                            const uint4 gw = *reinterpret_cast<const uint4 *>(p.gate + at);
+                            const uint32_t wd[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float gt = __uint_as_float((j & 1) ? (wd[j >> 1] & 0xffff0000u) : (wd[j >> 1] << 16));
+                                e[j] = __fdividef(e[j], 1.f + __expf(-gt));
+                            }
+                        }
+                        uint32_t r[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 t = __floats2bfloat162_rn(e[2 * j], e[2 * j + 1]);
+                            r[j] = *reinterpret_cast<const uint32_t *>(&t);
+                        }
+                        *reinterpret_cast<uint4 *>(p.out + at) = make_uint4(r[0], r[1], r[2], r[3]);
+                    }
+            } else {
+                float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.geo.rpg +
+                                       (size_t)h_of * p.geo.rpg + (rho - g.rho0)) * kRec;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4 *>(rec + 32 * c4 + 16 * half + 4 * i) =
+                            make_float4(o[4 * i][2 * hh + half], o[4 * i + 1][2 * hh + half],
+                                        o[4 * i + 2][2 * hh + half], o[4 * i + 3][2 * hh + half]);
+                if (c4 == 0) rec[kHD] = m[hh], rec[kHD + 1] = l[hh];
+            }
+        }
+    }
+}
+
+// Combines the partials that CTA range boundaries cut.  A block takes one (row, query head), or
+// blockDim / (32 * wpi) of them; wpi warps share one's partials (many CTAs on one sequence), each
+// 8 in flight, and join through shared memory.  Lane l takes dims 4l .. 4l + 3.
+constexpr int kMergeWarps = 8;
+__global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokParams p, int wpi) {
+    __shared__ float s_o[kMergeWarps][kHD], s_ml[kMergeWarps][2];
+    pdl_trigger();
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % wpi;
+    const int per = kMergeWarps / wpi, hb = (p.nh + per - 1) / per;
+    const int head = blockIdx.x % hb * per + warp / wpi;
+    const int j = blockIdx.x / hb, b = blockIdx.y;
+    const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0;
+    const bool in = head < p.nh && j < q_len;
+    const int kvh = in ? head / p.geo.gsz : 0, rho = j * p.geo.gsz + (in ? head % p.geo.gsz : 0);
+    const int v = b * p.geo.rgs + rho / p.geo.rpg;
+    const long long T = p.prefix_out[p.groups], P0 = in ? p.prefix_out[v] : 0, P1 = in ? p.prefix_out[v + 1] : 0;
+    int c0 = 0, c1 = -1;
+    if (P1 > P0) {
+        const int c = cta_of(lane == 0 ? P0 : P1 - 1, T, p.G);
+        c0 = __shfl_sync(0xffffffffu, c, 0), c1 = __shfl_sync(0xffffffffu, c, 1);
+    }
+    const bool cut = c1 > c0;  // else its one CTA wrote the output
+    const size_t rows = (size_t)p.hg * p.geo.rpg;
+    const float *base = p.part + ((size_t)(kvh / p.hg) * p.G * 2) * rows * kRec +
+                        ((size_t)(kvh % p.hg) * p.geo.rpg + rho % p.geo.rpg) * kRec;
+    constexpr int U = 8;
+    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+    if (cut)
+        for (int cb = c0 + sub * U; cb <= c1; cb += wpi * U) {
+            float m[U], l[U];
+            float4 o[U];
+            // lane u: the slot of CTA cb + u's partial (0 where the group starts in its range or
+            // fills its beginning), or none where its range is empty
+            int sl = -1;
+            if (lane < U && cb + lane <= c1) {
+                const long long lo = ((long long)(cb + lane) * T) / p.G, hi = ((long long)(cb + lane + 1) * T) / p.G;
+                if (hi > lo) sl = lo >= P0 ? 0 : 1;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int slot = __shfl_sync(0xffffffffu, sl, u);
+                m[u] = -INFINITY, l[u] = 0.f;
+                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (slot >= 0) {
+                    const float *rec = base + ((size_t)(cb + u) * 2 + slot) * rows * kRec;
+                    m[u] = __ldcg(rec + kHD);
+                    l[u] = __ldcg(rec + kHD + 1);
+                    o[u] = __ldcg(reinterpret_cast<const float4 *>(rec + 4 * lane));
+                }
+            }
+            float mc = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) mc = fmaxf(mc, m[u]);
+            if (mc == -INFINITY) continue;
+            const float f = ex2(M - mc);
+            L *= f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] *= f;
+            M = mc;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float w = l[u] * ex2(m[u] - M);
+                L += w;
+                O[0] += w * o[u].x, O[1] += w * o[u].y, O[2] += w * o[u].z, O[3] += w * o[u].w;
+            }
+        }
+    if (wpi > 1) {
+        *reinterpret_cast<float4 *>(&s_o[warp][4 * lane]) = make_float4(O[0], O[1], O[2], O[3]);
+        if (lane == 0) s_ml[warp][0] = M, s_ml[warp][1] = L;
+        __syncthreads();
+        if (sub) return;
+        float mc = M;
+        for (int w = 1; w < wpi; ++w) mc = fmaxf(mc, s_ml[warp + w][0]);
+        const float mb = mc == -INFINITY ? 0.f : mc;
+        const float f = ex2(M - mb);
+        L *= f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) O[e] *= f;
+        for (int w = 1; w < wpi; ++w) {
+            const float g = ex2(s_ml[warp + w][0] - mb);
+            L += s_ml[warp + w][1] * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] += g * s_o[warp + w][4 * lane + e];
+        }
+    }
+    if (!cut) return;
+    const size_t ob = ((size_t)(q0 + j) * p.nh + head) * kHD + 4 * lane;
+    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
+    uint2 gw = make_uint2(0u, 0u);
+    if (p.gate) gw = *reinterpret_cast<const uint2 *>(p.gate + ob);
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[i] = O[i] * f;
+        if (p.gate) {
+            const uint32_t w = i < 2 ? gw.x : gw.y;
+            const float gt = __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+            e[i] = __fdividef(e[i], 1.f + __expf(-gt));
+        }
+    }
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0], e[1]), hi = __floats2bfloat162_rn(e[2], e[3]);
+    *reinterpret_cast<uint2 *>(p.out + ob) =
+        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+
+// ---------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------
+struct TokPlan {
+    int hg, ngroups, ch, kw, pps, rpg, rgs, G, stages, seqs_per_launch;
+    size_t stage_bytes, smem, part_bytes, prefix_bytes;
+};
+
+constexpr size_t kTokSmem = 200 * 1024;  // ring; with the static arrays below the 227 KB of an SM
+
+TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks) {
+    TokPlan t;
+    const int nkv = (int)d->n_kv_heads, gsz = (int)(d->n_heads / d->n_kv_heads);
+    const long long max_q = (long long)(d->max_q_len < 1 ? 1 : (d->max_q_len < d->total_q ? d->max_q_len : d->total_q));
+    const long long rows = max_q * gsz;
+    // row tiles first (they share the pages a CTA reads), then as many KV heads as fill the warps
+    t.ch = (int)(rows > 16 * kTokWarps ? kTokWarps : (rows + 15) / 16);
+    const int most = kTokWarps / t.ch;
+    t.ngroups = (nkv + most - 1) / most;
+    t.hg = (nkv + t.ngroups - 1) / t.ngroups;
+    t.kw = kTokWarps / (t.hg * t.ch);
+    t.pps = 2 * t.kw;
+    t.rpg = 16 * t.ch;
+    t.rgs = (int)((rows + t.rpg - 1) / t.rpg);
+    t.seqs_per_launch = t.rgs >= kTokGroups ? 1 : kTokGroups / t.rgs;
+    t.stage_bytes = (size_t)t.pps * t.hg * 4096;
+    const size_t join = t.kw > 1 && t.ch > 1 ? (size_t)t.hg * t.ch * 16 * kRec * sizeof(float) : 0;
+    t.stages = (int)((kTokSmem - join) / t.stage_bytes);
+    if (t.stages > kTokStages) t.stages = kTokStages;
+    t.smem = t.stages * t.stage_bytes + join + 1024;
+    // one CTA per SM over the head groups, but no more than leaves each a few blocks by the
+    // host's bound on the batch's pages
+    long long keys = (long long)d->max_context;
+    if (window > 0) {
+        const long long seen = (long long)window + (long long)sinks + max_q + 32;
+        if (seen < keys && window < (1u << 30) && sinks < (1u << 30)) keys = seen;
+    }
+    const long long blocks = (long long)d->num_seqs * t.rgs * ((keys + 16 * t.pps - 1) / (16 * t.pps));
+    const int per = num_sms() / t.ngroups < 1 ? 1 : num_sms() / t.ngroups;
+    const long long want = (blocks + 3) / 4;
+    t.G = (int)(want < 1 ? 1 : (want < per ? want : per));
+    t.part_bytes = (size_t)t.ngroups * t.G * 2 * t.hg * t.rpg * kRec * sizeof(float);
+    t.prefix_bytes = (size_t)(kTokGroups + 4) * sizeof(int);
+    return t;
+}
+
+int encode_pages(const uint8_t *kc, const uint8_t *vc, int nkv, int num_blocks, int hg, CUtensorMap (&maps)[2],
+                 const char *what) {
+    TensorMapEncodeTiledFn enc = tensor_map_encoder();
+    PILM_REQUIRE(enc, ECPU_ERR_UNSUPPORTED, "%s: cuTensorMapEncodeTiled is unavailable", what);
+    const uint8_t *src[2] = {kc, vc};
+    for (int i = 0; i < 2; ++i) {
+        // (dim, slot, head): a box of 128 x 16 x hg lands as [head][slot][128 B], each head's 2 KB
+        // a SWIZZLE_128B tile
+        cuuint64_t dims[3] = {(cuuint64_t)kHD, (cuuint64_t)num_blocks * kKv8Page, (cuuint64_t)nkv};
+        cuuint64_t strides[2] = {(cuuint64_t)nkv * kHD, (cuuint64_t)kHD};
+        cuuint32_t box[3] = {(cuuint32_t)kHD, (cuuint32_t)kKv8Page, (cuuint32_t)hg};
+        cuuint32_t es[3] = {1, 1, 1};
+        const CUresult r = enc(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, (void *)src[i], dims, strides, box, es,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        PILM_REQUIRE(r == CUDA_SUCCESS, ECPU_ERR_PARAM, "%s: the cache's tensor map was rejected (error %d)", what,
+                     (int)r);
+    }
+    return ECPU_OK;
+}
+
+int check_error(const char *what) {
+    if (!sync_mode() || capturing()) return ECPU_OK;
+    int *word = nullptr;
+    if (cudaGetSymbolAddress((void **)&word, g_kv8_error) != cudaSuccess) return ECPU_OK;
+    return check_error_word_at(word, what, "a wait for a page did not complete");
 }
 
 }  // namespace
@@ -81,8 +847,9 @@ extern "C" {
 
 size_t ekernel_paged_attention_kv8_workspace_bytes(const ekernel_paged_attn_desc_t *desc, size_t window,
                                                    size_t sinks) {
-    (void)window, (void)sinks;
-    return kv8_check_desc(desc, "ekernel_paged_attention_kv8_workspace_bytes") == ECPU_OK ? 256 : 0;
+    if (kv8_check_desc(desc, "ekernel_paged_attention_kv8_workspace_bytes") != ECPU_OK) return 0;
+    const TokPlan t = plan_tokens(desc, window, sinks);
+    return t.part_bytes + t.prefix_bytes;
 }
 
 int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, const uint16_t *q,
@@ -99,22 +866,62 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
     PILM_REQUIRE(!desc->output_gate || gate, ECPU_ERR_PARAM, "%s: gate required when output_gate", what);
     PILM_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out | (uintptr_t)gate) & 15) == 0,
                  ECPU_ERR_PARAM, "%s: the caches, q, gate and out must be 16-byte aligned", what);
-    const size_t need = ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks);
+    const TokPlan t = plan_tokens(desc, window, sinks);
+    const size_t need = t.part_bytes + t.prefix_bytes;
     PILM_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, ECPU_ERR_PARAM,
                  "%s: workspace must be 16-byte aligned and hold %zu bytes, got %zu", what, need, workspace_bytes);
-    AttnParams p;
-    p.q = (const __nv_bfloat16 *)q;
-    p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
-    p.kc = k_cache, p.vc = v_cache, p.ks = k_scale, p.vs = v_scale;
-    p.block_table = block_table, p.cu_q = cu_q, p.ctx = context_lens;
-    p.out = (__nv_bfloat16 *)out;
-    p.nh = (int)desc->n_heads, p.nkv = (int)desc->n_kv_heads, p.num_seqs = (int)desc->num_seqs;
-    p.max_blocks = (int)desc->max_blocks_per_seq, p.num_blocks = (int)desc->num_blocks;
-    p.window = (long long)window, p.sinks = (long long)sinks;
-    p.scale = 0.08838834764831845f;
-    const size_t items = desc->total_q * desc->n_heads;
-    launch_pdl(kv8_attn_simple, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, p, (int)desc->total_q);
-    return check_launch(what);
+    CUtensorMap maps[2];
+    rc = encode_pages(k_cache, v_cache, (int)desc->n_kv_heads, (int)desc->num_blocks, t.hg, maps, what);
+    if (rc != ECPU_OK) return rc;
+    cudaFuncSetAttribute(kv8_attn_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTokSmem + 1024));
+    for (size_t b0 = 0; b0 < desc->num_seqs; b0 += (size_t)t.seqs_per_launch) {
+        const int seqs = (int)(desc->num_seqs - b0 < (size_t)t.seqs_per_launch ? desc->num_seqs - b0
+                                                                               : (size_t)t.seqs_per_launch);
+        TokParams p;
+        p.geo.cu_q = cu_q + b0;
+        p.geo.ctx = context_lens + b0;
+        p.geo.gsz = (int)(desc->n_heads / desc->n_kv_heads);
+        p.geo.rpg = t.rpg;
+        p.geo.rgs = t.rgs;
+        const size_t cap = 1u << 30;  // positions stay below it: a larger window is none
+        p.geo.window = window >= cap ? 0 : (int)window;
+        p.geo.sinks = (int)(sinks < cap ? sinks : cap);
+        p.q = (const __nv_bfloat16 *)q;
+        p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
+        p.ks = k_scale;
+        p.vs = v_scale;
+        p.block_table = block_table + b0 * desc->max_blocks_per_seq;
+        p.out = (__nv_bfloat16 *)out;
+        p.part = (float *)workspace;
+        p.prefix_out = (int *)((char *)workspace + t.part_bytes);
+        p.nh = (int)desc->n_heads;
+        p.nkv = (int)desc->n_kv_heads;
+        p.max_blocks = (int)desc->max_blocks_per_seq;
+        p.num_blocks = (int)desc->num_blocks;
+        p.groups = seqs * t.rgs;
+        p.hg = t.hg;
+        p.ch = t.ch;
+        p.kw = t.kw;
+        p.pps = t.pps;
+        p.stages = t.stages;
+        p.G = t.G;
+        launch_pdl(kv8_attn_tokens, dim3((unsigned)t.G, (unsigned)t.ngroups), dim3((t.hg * t.ch * t.kw + 1) * 32), t.smem,
+                   maps[0], maps[1], p);
+        rc = check_launch(what);
+        if (rc != ECPU_OK) return rc;
+        rc = check_error(what);
+        if (rc != ECPU_OK) return rc;
+        if (t.G == 1) continue;  // every group whole
+        // a row of the batch is the longest a sequence can have
+        const int max_q = (int)(desc->max_q_len < 1 ? 1 : (desc->max_q_len < desc->total_q ? desc->max_q_len : desc->total_q));
+        const int wpi = t.G > 16 * seqs * t.rgs ? kMergeWarps : 1;
+        const int per = kMergeWarps / wpi;
+        launch_pdl(kv8_attn_merge, dim3((unsigned)((p.nh + per - 1) / per * max_q), (unsigned)seqs),
+                   dim3(kMergeWarps * 32), 0, p, wpi);
+        rc = check_launch(what);
+        if (rc != ECPU_OK) return rc;
+    }
+    return ECPU_OK;
 }
 
 }  // extern "C"

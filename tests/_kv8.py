@@ -66,13 +66,15 @@ def store(x, slots, codes, scale):
 
 
 def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None, window=0, sinks=0):
-    """float64 outputs [T, nh * 128], and the bound's parts: sum p |v| (same shape) and the
-    largest sum |q k| / sqrt(128) of each row and head [T, nh]."""
+    """float64 outputs [T, nh * 128], and the bound's parts: sum p |v| (same shape), and of each
+    row and head [T, nh] the largest sum |q k| / sqrt(128) and the number of keys times the
+    largest value its V scales allow (448 * scale)."""
     T, nh = q.shape[0], q.shape[1] // HD
     g, dev, blocks = nh // nkv, q.device, codes_k.shape[0]
     out = torch.zeros((T, nh, HD), dtype=torch.float64, device=dev)
     pv = torch.zeros_like(out)
     sb = torch.zeros((T, nh), dtype=torch.float64, device=dev)
+    vt = torch.zeros((T, nh), dtype=torch.float64, device=dev)
     r0 = 0
     for b, (n, ctx) in enumerate(zip(q_lens, ctxs)):
         rows, r0 = slice(r0, r0 + n), r0 + n
@@ -87,6 +89,8 @@ def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None,
             v = torch.where(ok[:, None, None, None], v, torch.zeros_like(v))
             return v.flatten(0, 1)[:ctx].transpose(0, 1)                 # [kv, ctx, 128]
         k, v = gather(codes_k, ks), gather(codes_v, vs)
+        top = torch.where(ok[:, None], vs[at].double(), 0.0).amax(0)
+        vt[rows] = (ctx * 448.0 * top).repeat_interleave(g)
         pos = torch.arange(ctx - n, ctx, device=dev)[:, None]
         key = torch.arange(ctx, device=dev)[None]
         seen = key <= pos
@@ -107,7 +111,7 @@ def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None,
     if gate is not None:
         sg = torch.sigmoid(gate.double()).view(T, nh, HD)
         out, pv = out * sg, pv * sg
-    return out.view(T, nh * HD), pv.view(T, nh * HD), sb
+    return out.view(T, nh * HD), pv.view(T, nh * HD), (sb, vt)
 
 
 def assert_attention(got, ref, pv, sb, max_ctx):
@@ -118,10 +122,15 @@ def assert_attention(got, ref, pv, sb, max_ctx):
                                                  fp32 sum of 128 products and its scaling
                                   + 2^-18        exp, division, the gate's sigmoid
                                   + ctx 2^-24    the fp32 sum over the keys)
+                    + keys * 448 * scale * 2^-39 a probability p is held as 2^14 p in f16, so the
+                                                 spacing of f16 below its normal range, 2^-24,
+                                                 leaves p at most 2^-39 off, whatever p
                     + 2^-126                     results below the normal range."""
+    sb, vt = sb
     T, nh = sb.shape
     e = 2 * 130 * 2.0 ** -24 * sb[:, :, None].expand(T, nh, HD).reshape(T, nh * HD)
     tol = 2.0 ** -8 * ref.abs() + pv * (2.0 ** -11 + e.clamp(max=2) + 2.0 ** -18 + max_ctx * 2.0 ** -24) + 2.0 ** -126
+    tol = tol + vt[:, :, None].expand(T, nh, HD).reshape(T, nh * HD) * 2.0 ** -39
     bad = ~((got.double() - ref).abs() <= tol)
     assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} values off, first at {bad.nonzero()[0].tolist()}: "
                            f"{got[bad][0].item()} for {ref[bad][0].item()}")
