@@ -87,9 +87,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
-// Probabilities are held as 2^14 exp(s - max), so that their f16 rounding keeps 11 bits down to
-// 2^-28 of the largest and drops nothing above 2^-39: a long tail of small ones still counts.
-constexpr float kProbBits = 14.f;
+// Probabilities are held as 2^9 exp(s - m) in f16 for a reference m at most kLag below the running
+// maximum (in base 2): at most 2^15, with 11 bits down to 2^-23 of exp(m) and steps of 2^-33 below,
+// so a long tail of small ones still counts.  The lag spares most of the rescalings of O: a new
+// maximum within it leaves m where it is.
+constexpr float kProbBits = 9.f, kLag = 6.f;
 
 // ---------------------------------------------------------------------------------
 // Geometry shared by the kernels.  A batch's rows are cut into groups: group (b, rg) holds the
@@ -149,9 +151,9 @@ __device__ __forceinline__ int cta_of(long long x, long long T, int G) {
 // TMA ring, and consumer warp (h, c, k) takes head h, row tile c (16 rows) and pages 2k, 2k + 1
 // of each block, so every byte is read from HBM once and 8 warps share the conversions.
 //
-// Per pair of pages a warp computes S = Q K8^T and O += P V8 with mma.sync m16n8k16 on f16: the
-// codes are converted in registers as they leave shared memory (two per instruction).  Both
-// products sum over an index whose order is free, and each order is chosen so that a thread's
+// Per pair of pages a warp computes S = Q K8^T with mma.sync m16n8k32 on the codes as they are
+// (the queries split into two e4m3 parts), and O += P V8 with m16n8k16 on f16 (P needs f16's
+// range; V's codes are converted in registers as they leave shared memory).  Both products sum over an index whose order is free, and each order is chosen so that a thread's
 // operand is contiguous in the cache as it lies there: thread (g, c) = (lane / 4, lane % 4) holds
 // dims 32c .. 32c + 31 of a key for S, and dims 16g .. 16g + 15 of its four keys for O, where
 // four byte permutes pair the keys.  With the TMA's 128-byte swizzle all these 16-byte
@@ -161,6 +163,10 @@ __device__ __forceinline__ int cta_of(long long x, long long T, int G) {
 // 128 rows.  mma.sync at 16 rows keeps up with HBM.
 // ---------------------------------------------------------------------------------
 constexpr int kTokWarps = 8;      // consumer warps at most
+// Three warpgroups: two of consumers, and one whose first warp is the producer.  Launched with
+// 168 registers a thread (64512 in all), the producer's group keeps 40 and the consumers take 232:
+// 256 * 232 + 128 * 40 = 64512.
+constexpr int kTokThreads = 384;
 constexpr int kTokGroups = 4096;  // groups per launch (their prefix is kept in shared memory)
 constexpr int kTokStages = 8;     // ring stages at most
 constexpr int kRec = kHD + 4;     // a partial: O[128] normalised, max (base 2), sum, two pad floats
@@ -187,7 +193,7 @@ __device__ void zero_rows(const TokParams &p, const Group &g, int head0, int hea
     }
 }
 
-__global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_constant__ CUtensorMap kmap,
                                                                            const __grid_constant__ CUtensorMap vmap,
                                                                            const TokParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -247,8 +253,10 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
     }
     const uint32_t ring = smem_u32(smem);
 
-    if (warp == consumers) {
+    if (warp >= kTokWarps) {
         // ---- producer ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp > kTokWarps) return;
         int v = v_first, issued = 0;
         Group g = group_of(p.geo, v);
         bool ok = true;
@@ -305,7 +313,8 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
             }
         return;
     }
-    if (warp > consumers) return;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    if (warp >= consumers) return;
 
     // ---- consumer warp (h, c, k) ----
     const int k_of = warp % p.kw, c_of = warp / p.kw % p.ch, h_of = warp / (p.kw * p.ch);
@@ -314,16 +323,9 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
     const bool head_ok = head < p.nkv;
     // byte offsets of this thread's loads in one head's 2 KB tile (rows of 128 B, 16-byte chunk i
     // of row r at i ^ (r & 7))
-    uint32_t k_off[2][2], v_off[4];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) k_off[t][i] = (8 * t + g4) * 128 + (((2 * c4 + i) ^ g4) << 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 2 * c4 + (i & 1) + 8 * (i >> 1);
-        v_off[i] = row * 128 + ((g4 ^ (row & 7)) << 4);
-    }
+    const uint32_t k_off = g4 * 128 + ((2 * c4 ^ g4) << 4);                    // key g4; its second chunk: ^ 16
+    const uint32_t v_off = 2 * c4 * 128 + ((g4 ^ (2 * c4)) << 4);              // key 2 c4
+    const uint32_t v_off1 = (2 * c4 + 1) * 128 + ((g4 ^ (2 * c4 + 1)) << 4);   // key 2 c4 + 1; both: + 8 rows
     // all consumer warps meet (bounded, unlike a hardware barrier whose partner has given up)
     int met = 0;
     auto meet = [&]() {
@@ -349,8 +351,8 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
         const bool active = head_ok && tile0 < g.rho1;
         const int tile1 = min(g.rho1, tile0 + 16);
 
-        // queries: row r in f16 as q * 2^k, the largest magnitude in [2^14, 2^15).  Exact for bf16
-        // elements down to 2^-29 of the largest; 2^-k goes into the row's score factor.
+        // queries in f16 as q * 2^k, the largest magnitude of the row in [2^14, 2^15): exact for bf16
+        // elements down to 2^-28 of the largest; 2^-k goes into the row's score factor
         uint32_t qf[8][4];
         float rowf[2];
         int qpos[2];
@@ -359,24 +361,18 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
             const int rho = tile0 + g4 + 8 * hh;
             const bool in = active && rho < tile1;
             qpos[hh] = in ? g.p0 + rho / p.geo.gsz : -1;
-            float e[32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (in)
-                    w = *reinterpret_cast<const uint4 *>(
-                        p.q + ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD +
-                        32 * c4 + 8 * i);
-                const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    e[8 * i + 2 * j] = __uint_as_float(wd[j] << 16);
-                    e[8 * i + 2 * j + 1] = __uint_as_float(wd[j] & 0xffff0000u);
-                }
-            }
+            const __nv_bfloat16 *qr =
+                p.q + ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD + 32 * c4;
+            uint4 w[4];
             float mx = 0.f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fabsf(e[i]));
+            for (int i = 0; i < 4; ++i) {
+                w[i] = in ? *reinterpret_cast<const uint4 *>(qr + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t wd[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(wd[j] << 16)), fabsf(__uint_as_float(wd[j] & 0xffff0000u))));
+            }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             int sh = 14 - ((int)(__float_as_uint(mx) >> 23) - 127);
@@ -384,13 +380,22 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
             const float up = pow2f(sh);
             rowf[hh] = pow2f(-sh) * kScoreScale;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                qf[s][hh] = pack_f16(e[4 * s] * up, e[4 * s + 1] * up);
-                qf[s][2 + hh] = pack_f16(e[4 * s + 2] * up, e[4 * s + 3] * up);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t wd[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    qf[2 * i + (j >> 1)][2 * (j & 1) + hh] =
+                        pack_f16(__uint_as_float(wd[j] << 16) * up, __uint_as_float(wd[j] & 0xffff0000u) * up);
             }
         }
-        // positions of the tile's first and last rows: pages every row sees whole need no mask
+        // The pages [plain0, plain1) of the list need no mask: every row of the tile sees them whole.
         const int pmin = g.p0 + tile0 / p.geo.gsz, pmax = g.p0 + (tile1 - 1) / p.geo.gsz;
+        int plain0 = 0, plain1 = pmin + 1 > 0 ? (pmin + 1) >> 4 : 0;  // ends at or before pmin
+        if (p.geo.window > 0) {
+            const int first = pmax - p.geo.window + 1;  // the last row's first key
+            plain0 = g.n_sink + max(0, (first > 0 ? (first + 15) >> 4 : 0) - g.lo_page);
+            plain1 = plain1 - g.lo_page + g.n_sink;
+        }
 
         float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f, inv_vref = 0.f;
 #pragma unroll
@@ -413,89 +418,96 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
             if (active && vp < g.nv) {
                 const uint32_t kb = ring + st * stage_bytes + (2 * k_of) * page_bytes + h_of * 2048;
                 const uint32_t vb = kb + p.pps * page_bytes;
-                const uint32_t valid = s_valid[st] >> (2 * k_of);
+                const uint32_t valid = s_valid[st] >> (2 * k_of) & 3u;
+                const bool masked = vp < plain0 || vp + 2 > plain1 || valid != 3u;
                 float kf[2], vf[2];
-                int key0[2];
-                bool masked = vp + 1 >= g.nv || (valid & 3u) != 3u;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int at = (2 * k_of + i) * p.hg + h_of;
                     kf[i] = s_scale[st][0][at];
                     vf[i] = s_scale[st][1][at];
-                    if (!((valid >> i) & 1u)) kf[i] = vf[i] = 0.f;
-                    key0[i] = page_of(g, vp + i) * 16;
-                    masked |= key0[i] + 15 > pmin ||
-                              (p.geo.window > 0 && key0[i] <= pmax - p.geo.window && key0[i] + 15 >= p.geo.sinks);
                 }
                 // ---- S = Q K8^T: two pages of two 8-key tiles, four independent chains ----
                 float s[2][2][4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t w[2][8];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const uint4 r = lds128(kb + i * page_bytes + k_off[t][hf]);
-                            w[t][4 * hf] = r.x, w[t][4 * hf + 1] = r.y, w[t][4 * hf + 2] = r.z, w[t][4 * hf + 3] = r.w;
-                        }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[i][t][j] = 0.f;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-                            mma_f16(s[i][t], qf[k], e4m3x2_to_f16x2(w[t][k]), e4m3x2hi_to_f16x2(w[t][k]));
-                }
-                // ---- scores in base 2, masks, online softmax ----
-                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float &e = s[i][t][j];
-                            e *= rowf[j >> 1] * kf[i];
-                            if (masked) {
+                        for (int j = 0; j < 4; ++j) s[i][t][j] = 0.f;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint4 w[2][2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+                            w[i][t] = lds128(kb + i * page_bytes + t * 1024 + (hf ? k_off ^ 16u : k_off));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int t = 0; t < 2; ++t) {
+                                const uint32_t c = k == 0 ? w[i][t].x : (k == 1 ? w[i][t].y : (k == 2 ? w[i][t].z : w[i][t].w));
+                                mma_f16(s[i][t], qf[4 * hf + k], e4m3x2_to_f16x2(c), e4m3x2hi_to_f16x2(c));
+                            }
+                }
+                // ---- scores in base 2, masks, online softmax ----
+                int key0[2] = {0, 0};
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const bool ok_page = (valid >> i) & 1u;
+                        if (!ok_page) kf[i] = vf[i] = 0.f;
+                        key0[i] = page_of(g, vp + i) * 16;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
                                 const int key = key0[i] + 8 * t + 2 * c4 + (j & 1), qp = qpos[j >> 1];
                                 const bool see = vp + i < g.nv && key <= qp &&
                                                  (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
-                                if (!((valid >> i) & 1u)) e = 0.f;  // a page of zeros
-                                if (!see) e = -INFINITY;
+                                // a page with no valid id is one of zeros
+                                s[i][t][j] = see ? (ok_page ? s[i][t][j] * (rowf[j >> 1] * kf[i]) : 0.f) : -INFINITY;
                             }
-                            mx[j >> 1] = fmaxf(mx[j >> 1], e);
-                        }
-                const float vtop = fmaxf(vref, fmaxf(vf[0], vp + 1 < g.nv ? vf[1] : 0.f));
-                float fac[2], base[2];
-                bool moved = vtop != vref;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float f[2] = {rowf[0] * kf[i], rowf[1] * kf[i]};
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[i][t][j] *= f[j >> 1];
+                    }
+                }
+                float mx[2];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
+                    mx[hh] = fmaxf(fmaxf(fmaxf(s[0][0][2 * hh], s[0][0][2 * hh + 1]), fmaxf(s[0][1][2 * hh], s[0][1][2 * hh + 1])),
+                                   fmaxf(fmaxf(s[1][0][2 * hh], s[1][0][2 * hh + 1]), fmaxf(s[1][1][2 * hh], s[1][1][2 * hh + 1])));
                     mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
                     mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
-                    const float mn = fmaxf(m[hh], mx[hh]);
-                    moved |= mn != m[hh];
-                    const float mb = mn == -INFINITY ? 0.f : mn;
-                    fac[hh] = ex2(m[hh] - mb);
-                    base[hh] = kProbBits - mb;
-                    m[hh] = mn;
                 }
-                if (__any_sync(0xffffffffu, moved)) {  // a running maximum, or the V scale's, rose
-                    l[0] *= fac[0], l[1] *= fac[1];
-                    if (vtop != vref) {
-                        const float f = vref * (vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f);
-                        fac[0] *= f, fac[1] *= f;
-                        vref = vtop;
-                        inv_vref = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
-                    }
+                const float vtop = fmaxf(vref, fmaxf(vf[0], vf[1]));
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || vtop > vref)) {
+                    const float inv = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
+                    const float vfac = vref * inv;
+                    vref = vtop, inv_vref = inv;
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) {
-                        o[n][0] *= fac[0], o[n][1] *= fac[0];
-                        o[n][2] *= fac[1], o[n][3] *= fac[1];
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const float mn = fmaxf(m[hh], mx[hh]);
+                        const float f = mn == m[hh] ? 1.f : ex2(m[hh] - mn);  // first keys: ex2(-inf) = 0
+                        m[hh] = mn;
+                        l[hh] *= f;
+                        const float fo = f * vfac;
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) o[n][2 * hh] *= fo, o[n][2 * hh + 1] *= fo;
                     }
                 }
+                const float base[2] = {m[0] == -INFINITY ? 0.f : kProbBits - m[0],
+                                       m[1] == -INFINITY ? 0.f : kProbBits - m[1]};
                 uint32_t pa[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__((kTokWarps + 1) * 32, 1) kv8_attn_tokens(const
                 for (int i = 0; i < 2; ++i) {
                     uint4 w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) w[k] = lds128(vb + i * page_bytes + v_off[k]);
+                    for (int k = 0; k < 4; ++k) w[k] = lds128(vb + i * page_bytes + (k >> 1) * 1024 + (k & 1 ? v_off1 : v_off));
                     if (masked) {  // bytes of keys that no row sees may be NaN codes: P = 0 there
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
@@ -905,7 +917,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.pps = t.pps;
         p.stages = t.stages;
         p.G = t.G;
-        launch_pdl(kv8_attn_tokens, dim3((unsigned)t.G, (unsigned)t.ngroups), dim3((t.hg * t.ch * t.kw + 1) * 32), t.smem,
+        launch_pdl(kv8_attn_tokens, dim3((unsigned)t.G, (unsigned)t.ngroups), dim3(kTokThreads), t.smem,
                    maps[0], maps[1], p);
         rc = check_launch(what);
         if (rc != ECPU_OK) return rc;

@@ -67,14 +67,14 @@ def store(x, slots, codes, scale):
 
 def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None, window=0, sinks=0):
     """float64 outputs [T, nh * 128], and the bound's parts: sum p |v| (same shape), and of each
-    row and head [T, nh] the largest sum |q k| / sqrt(128) and the number of keys times the
+    row and head [T, nh] the largest sum |q k| / sqrt(128), the largest max|q| sum |k| / sqrt(128), and the number of keys times the
     largest value its V scales allow (448 * scale)."""
     T, nh = q.shape[0], q.shape[1] // HD
     g, dev, blocks = nh // nkv, q.device, codes_k.shape[0]
     out = torch.zeros((T, nh, HD), dtype=torch.float64, device=dev)
     pv = torch.zeros_like(out)
     sb = torch.zeros((T, nh), dtype=torch.float64, device=dev)
-    vt = torch.zeros((T, nh), dtype=torch.float64, device=dev)
+    vt, qk = torch.zeros_like(sb), torch.zeros_like(sb)
     r0 = 0
     for b, (n, ctx) in enumerate(zip(q_lens, ctxs)):
         rows, r0 = slice(r0, r0 + n), r0 + n
@@ -101,6 +101,8 @@ def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None,
         sa = torch.einsum("nkgd,kcd->nkgc", qq.abs(), k.abs()) / math.sqrt(HD)
         m4 = seen[:, None, None]
         s = torch.where(m4, s, torch.full_like(s, -math.inf))
+        ka = torch.where(m4, k.abs().sum(-1)[None, :, None], torch.zeros_like(sa)).amax(-1) / math.sqrt(HD)
+        qk[rows] = (qq.abs().amax(-1) * ka).reshape(n, nh)
         mx = s.amax(-1, keepdim=True)
         p = torch.where(m4, torch.exp(s - torch.where(mx.isfinite(), mx, torch.zeros_like(mx))), torch.zeros_like(s))
         tot = p.sum(-1, keepdim=True)
@@ -111,26 +113,31 @@ def attention(q, codes_k, codes_v, ks, vs, tables, q_lens, ctxs, nkv, gate=None,
     if gate is not None:
         sg = torch.sigmoid(gate.double()).view(T, nh, HD)
         out, pv = out * sg, pv * sg
-    return out.view(T, nh * HD), pv.view(T, nh * HD), (sb, vt)
+    return out.view(T, nh * HD), pv.view(T, nh * HD), (sb, qk, vt)
 
 
 def assert_attention(got, ref, pv, sb, max_ctx):
     """|got - ref| <= 2^-8 |ref| (the output's rounding to bf16)
                     + sum p|v| * (2^-11          probabilities rounded to f16
                                   + 2 e          a score off by e moves its probability and the
-                                                 sum by e each; e = 130 * 2^-24 * sum|q k|, the
-                                                 fp32 sum of 128 products and its scaling
+                                                 sum by e each; e = 260 * 2^-24 * sum|q k| (the
+                                                 sums of 128 products each, which the tensor
+                                                 cores truncate at 2^-23, and their scaling)
+                                                 + 2^-39 * max|q| * sum|k| (a query is held in
+                                                 f16 with its largest element at least 2^14: the
+                                                 steps of 2^-24 below the normal range)
                                   + 2^-18        exp, division, the gate's sigmoid
                                   + ctx 2^-24    the fp32 sum over the keys)
-                    + keys * 448 * scale * 2^-39 a probability p is held as 2^14 p in f16, so the
-                                                 spacing of f16 below its normal range, 2^-24,
-                                                 leaves p at most 2^-39 off, whatever p
+                    + keys * 448 * scale * 2^-34 a probability p (the largest: at least 1) is held
+                                                 as 2^9 p in f16: the steps of 2^-24 below the
+                                                 normal range leave it at most 2^-34 off
                     + 2^-126                     results below the normal range."""
-    sb, vt = sb
+    sb, qk, vt = sb
+    full = lambda x: x[:, :, None].expand(T, nh, HD).reshape(T, nh * HD)  # noqa: E731
     T, nh = sb.shape
-    e = 2 * 130 * 2.0 ** -24 * sb[:, :, None].expand(T, nh, HD).reshape(T, nh * HD)
+    e = 2 * full(260 * 2.0 ** -24 * sb + 2.0 ** -39 * qk)
     tol = 2.0 ** -8 * ref.abs() + pv * (2.0 ** -11 + e.clamp(max=2) + 2.0 ** -18 + max_ctx * 2.0 ** -24) + 2.0 ** -126
-    tol = tol + vt[:, :, None].expand(T, nh, HD).reshape(T, nh * HD) * 2.0 ** -39
+    tol = tol + full(vt) * 2.0 ** -34
     bad = ~((got.double() - ref).abs() <= tol)
     assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} values off, first at {bad.nonzero()[0].tolist()}: "
                            f"{got[bad][0].item()} for {ref[bad][0].item()}")
