@@ -41,11 +41,11 @@ def table_of(b, width=None):
 def check_store(x, slots, before, scale_before, after, scale_after):
     """The cache after a call against exact rows x [T, kv, 128]: a new code is the nearest to its
     exact value, scales and kept codes are exact, everything else is unchanged.
-    Nearest up to the fp32 error of that value: the norm's ten roundings (the sum of squares
-    nine deep, halved by the root; root, division, two products) are 10 * 2^-24 of each value;
-    a rotation adds two products (one more rounding each) and rounds: 12 * 2^-24 * (|a| + |b|),
-    and |a| + |b| <= 2 sqrt(2) times the head's largest rotated value (a rotation keeps a pair's
-    norm), so 34 * 2^-24 < 2^-18 of that largest value."""
+    Nearest up to the fp32 error of that value: the norm's roundings (the sum of squares nine
+    deep, halved by the root; the reciprocal root, 2 units; three products) are 10 * 2^-24 of each
+    value; a rotation adds two products (one more rounding each) and rounds: 12 * 2^-24 *
+    (|a| + |b|), and |a| + |b| <= 2 sqrt(2) times the head's largest rotated value (a rotation
+    keeps a pair's norm), so 34 * 2^-24 < 2^-18 of that largest value."""
     val, sc = ref.store(x, slots, before, scale_before)
     assert torch.equal(scale_after.double().nan_to_num(-1), sc.nan_to_num(-1))
     blocks, _, nkv, _ = before.shape
