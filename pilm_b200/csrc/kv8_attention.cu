@@ -93,6 +93,44 @@ constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // lo
 // maximum within it leaves m where it is.
 constexpr float kProbBits = 9.f, kLag = 6.f;
 
+// x / (1 + exp(-gate)) of eight outputs
+__device__ __forceinline__ void apply_gate(float (&e)[8], const __nv_bfloat16 *gate) {
+    const uint4 gw = *reinterpret_cast<const uint4 *>(gate);
+    const uint32_t wd[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float gt = __uint_as_float((j & 1) ? (wd[j >> 1] & 0xffff0000u) : (wd[j >> 1] << 16));
+        e[j] = __fdividef(e[j], 1.f + __expf(-gt));
+    }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *out, const float (&e)[8]) {
+    uint32_t r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(e[2 * j], e[2 * j + 1]);
+        r[j] = *reinterpret_cast<const uint32_t *>(&t);
+    }
+    *reinterpret_cast<uint4 *>(out) = make_uint4(r[0], r[1], r[2], r[3]);
+}
+// four merged outputs o * f at element `at`
+__device__ __forceinline__ void finish4(__nv_bfloat16 *out, const __nv_bfloat16 *gate, size_t at, const float (&o)[4], float f) {
+    uint2 gw = make_uint2(0u, 0u);
+    if (gate) gw = *reinterpret_cast<const uint2 *>(gate + at);
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        e[i] = o[i] * f;
+        if (gate) {
+            const uint32_t w = i < 2 ? gw.x : gw.y;
+            const float gt = __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
+            e[i] = __fdividef(e[i], 1.f + __expf(-gt));
+        }
+    }
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0], e[1]), hi = __floats2bfloat162_rn(e[2], e[3]);
+    *reinterpret_cast<uint2 *>(out + at) =
+        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+}
+
 // ---------------------------------------------------------------------------------
 // Geometry shared by the kernels.  A batch's rows are cut into groups: group (b, rg) holds the
 // rows rho in [rg * rpg, (rg + 1) * rpg) of sequence b, rho = j * gsz + g for query row j and
@@ -640,22 +678,8 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                         float e[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) e[j] = o[8 * i + j][2 * hh + half];
-                        if (p.gate) {
-                            const uint4 gw = *reinterpret_cast<const uint4 *>(p.gate + at);
-                            const uint32_t wd[4] = {gw.x, gw.y, gw.z, gw.w};
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float gt = __uint_as_float((j & 1) ? (wd[j >> 1] & 0xffff0000u) : (wd[j >> 1] << 16));
-                                e[j] = __fdividef(e[j], 1.f + __expf(-gt));
-                            }
-                        }
-                        uint32_t r[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __nv_bfloat162 t = __floats2bfloat162_rn(e[2 * j], e[2 * j + 1]);
-                            r[j] = *reinterpret_cast<const uint32_t *>(&t);
-                        }
-                        *reinterpret_cast<uint4 *>(p.out + at) = make_uint4(r[0], r[1], r[2], r[3]);
+                        if (p.gate) apply_gate(e, p.gate + at);
+                        store8(p.out + at, e);
                     }
             } else {
                 float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.geo.rpg +
@@ -762,21 +786,549 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokPara
     if (!cut) return;
     const size_t ob = ((size_t)(q0 + j) * p.nh + head) * kHD + 4 * lane;
     const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
-    uint2 gw = make_uint2(0u, 0u);
-    if (p.gate) gw = *reinterpret_cast<const uint2 *>(p.gate + ob);
-    float e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        e[i] = O[i] * f;
-        if (p.gate) {
-            const uint32_t w = i < 2 ? gw.x : gw.y;
-            const float gt = __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
-            e[i] = __fdividef(e[i], 1.f + __expf(-gt));
+    finish4(p.out, p.gate, ob, O, f);
+}
+
+// ---------------------------------------------------------------------------------
+// Chunk kernel: prompts and other calls with many rows per KV head, bound by the tensor cores.
+//
+// A CTA owns 256 rows (two tiles of 128) of one KV head of one sequence and a range of its
+// 128-key blocks.  Four converter warps read a block's codes from the cache, write them to shared
+// memory as f16 (K and V each into two 32 KB stages; the code-to-f16 step is shared by both tiles),
+// and one thread issues, per block and tile,
+//   S = Q K8^T    8 x tcgen05.mma M=128 N=128 K=16 (kind::f16), both operands in shared memory
+//   O += P V8     8 x the same, P from TMEM, V as it lies (keys x dims, an MN-major operand)
+// Two groups of four softmax warps, a thread per row, turn S into P in place (P's 64 columns lie
+// over S's 128), so S, P and O of both tiles fill the 512 TMEM columns, and while one tile's
+// softmax runs the tensor cores work on the other tile.  The softmax takes the row maximum page by
+// page on the raw products (a page's scale is one factor) and folds the page's V scale into the
+// exponent: p' = 2^(s f + c), c = bits - m + log2(vs / vref), one fma and one exp2 per score.
+// Register split of the 512 threads (128 each at launch, 65536): 184 for the softmax warps, 104 for
+// the converters, 40 for the issuer's group: 256 * 184 + 128 * 104 + 128 * 40 = 65536.
+// ---------------------------------------------------------------------------------
+constexpr int kChThreads = 512;
+constexpr int kChTile = 128, kChRows = 2 * kChTile;  // rows per tile and per CTA
+constexpr int kChKeys = 128;                         // keys per block
+constexpr int kChHalf = kChKeys * 128;               // 64 dims of a 128-row f16 operand: 16 KB
+constexpr int kChOperand = 2 * kChHalf;              // 32 KB
+constexpr size_t kChSmemK = 2 * (size_t)kChOperand, kChSmemV = kChSmemK + 2 * (size_t)kChOperand;
+constexpr size_t kChSmem = kChSmemV + 2 * (size_t)kChOperand + 1024;
+constexpr int kChScales = 4;  // blocks whose scales are kept: the softmax may be two behind the copies
+
+struct ChunkParams {
+    Geometry geo;  // rpg = kChRows
+    const __nv_bfloat16 *q, *gate;
+    const uint8_t *kc, *vc;
+    const float *ks, *vs;
+    const int32_t *block_table;
+    __nv_bfloat16 *out;
+    float *part;  // [splits][total_q][nh][kRec], when splits > 1
+    int nh, nkv, max_blocks, num_blocks, total_q, splits;
+};
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// SWIZZLE_128B operand, 1024 bytes between groups of 8 rows (of 8 keys, for the MN-major V), and
+// for V kChHalf between the two halves of the dims
+__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)lead << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// two floats at once
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct __align__(8) ChunkBars {
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done;
+};
+
+// grid: (sequences x groups x splits, n_kv)
+__global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ ChunkBars bar;
+    __shared__ __align__(16) float s_scale[kChScales][2][8];  // [block][K, V][page]
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 8);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.k_full[i], 4);
+            mbar_init(&bar.k_empty[i], 1);
+            mbar_init(&bar.v_full[i], 4);
+            mbar_init(&bar.v_empty[i], 1);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 4);
+        }
+        mbar_init(&bar.o_done, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    pdl_wait();
+
+    // the last positions see the most keys: their groups first
+    const int split = blockIdx.x % p.splits, kvh = blockIdx.y;
+    const int seqs = (int)gridDim.x / (p.splits * p.geo.rgs);
+    const int gi = blockIdx.x / p.splits, b = gi % seqs, rg = p.geo.rgs - 1 - gi / seqs;
+    const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0, ctx = p.geo.ctx[b];
+    const int gsz = p.geo.gsz, p0 = ctx - q_len;
+    const int rho0 = rg * kChRows, rho1 = min(q_len * gsz, rho0 + kChRows);
+    const int tiles = rho1 - rho0 > kChTile ? 2 : (rho1 > rho0 ? 1 : 0);
+    // blocks of the group: n_sink from the first key on, then those from lo on
+    int n_sink = 0, lo = 0, nb = 0;
+    if (tiles > 0) {
+        const int pmin = p0 + rho0 / gsz, pmax = p0 + (rho1 - 1) / gsz;
+        if (pmax >= 0) {
+            if (p.geo.window > 0) {
+                lo = max(0, pmin - p.geo.window + 1) / kChKeys;
+                n_sink = min((p.geo.sinks + kChKeys - 1) / kChKeys, lo);
+            }
+            nb = n_sink + pmax / kChKeys + 1 - lo;
         }
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(e[0], e[1]), hi = __floats2bfloat162_rn(e[2], e[3]);
-    *reinterpret_cast<uint2 *>(p.out + ob) =
-        make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    const int j0 = (int)((long long)nb * split / p.splits), j1 = (int)((long long)nb * (split + 1) / p.splits);
+    auto key_of = [&](int j) { return (j < n_sink ? j : j - n_sink + lo) * kChKeys; };
+    // a wait of the whole warp; false once any lane gave up
+    auto wait = [&](uint64_t *m, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(m, parity, &s_abort));
+        if (!ok) *(volatile int *)&s_abort = 1;
+        return ok;
+    };
+
+    if (warp >= 12) {
+        // ---- issuer ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 12 && j0 < j1) {
+            const uint32_t idesc_s = (1u << 4) | ((uint32_t)(kChKeys >> 3) << 17) | ((uint32_t)(kChTile >> 4) << 24);
+            const uint32_t idesc_pv = idesc_s | (1u << 16);  // B MN-major
+            const uint32_t base = smem_u32(smem);
+            auto issue_s = [&](int t, int n) {  // block n of this CTA
+                if (lane == 0) {
+                    const uint32_t qa = base + t * kChOperand, ka = base + (uint32_t)kChSmemK + (n & 1) * kChOperand;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        tc_mma_ss(tmem + 128 * t, tc_desc(qa + (k >> 2) * kChHalf, 1) + 2 * (k & 3),
+                                  tc_desc(ka + (k >> 2) * kChHalf, 1) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+                    tc_commit(&bar.s_full[t]);
+                    if (t == tiles - 1) tc_commit(&bar.k_empty[n & 1]);
+                }
+                __syncwarp();
+            };
+            const int total = j1 - j0;
+            bool ok = wait(&bar.q_full, 0) && wait(&bar.k_full[0], 0);
+            if (ok) {
+                tc_fence_after();
+                for (int t = 0; t < tiles; ++t) issue_s(t, 0);
+            }
+            for (int n = 0; ok && n < total; ++n) {
+                ok = wait(&bar.v_full[n & 1], (uint32_t)(n >> 1) & 1u);
+                for (int t = 0; ok && t < tiles; ++t) {
+                    ok = wait(&bar.p_full[t], (uint32_t)n & 1u);
+                    if (ok && n + 1 < total && t == 0) ok = wait(&bar.k_full[(n + 1) & 1], (uint32_t)((n + 1) >> 1) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t va = base + (uint32_t)kChSmemV + (n & 1) * kChOperand;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+                            tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, tc_desc(va + k * 2048, kChHalf >> 4),
+                                      idesc_pv, n > 0 || k > 0 ? 1u : 0u);
+                        if (t == tiles - 1) tc_commit(&bar.v_empty[n & 1]);
+                    }
+                    __syncwarp();
+                    if (n + 1 < total) issue_s(t, n + 1);  // after PV: S lies over P
+                }
+            }
+            // everything issued has completed (also when a wait gave up)
+            if (lane == 0) tc_commit(&bar.o_done);
+            __syncwarp();
+            bool done = false;
+            for (uint32_t i = 0; i < kWaitLimit && !done; ++i) done = mbar_try_wait(&bar.o_done, 0);
+            if (!ok && lane == 0) atomicExch(&g_kv8_error, 1);
+            __syncwarp();
+        }
+    } else if (warp >= 8) {
+        // ---- converters: thread (row, ch) takes 16 codes of token `row` of each of a block's pages ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        const int tid = threadIdx.x - 256, row = tid >> 3, ch = tid & 7;
+        const int32_t *bt = p.block_table + (size_t)b * p.max_blocks;
+        // page ids of block j: lane i holds page i's
+        auto fetch_ids = [&](int j) {
+            int blk = -1;
+            if (j < j1 && lane < 8) {
+                const int pg = key_of(j) / kKv8Page + lane;
+                if (pg < p.max_blocks && pg * kKv8Page < ctx) blk = bt[pg];
+                if (blk < 0 || blk >= p.num_blocks) blk = -1;
+            }
+            return blk;
+        };
+        auto fetch = [&](const uint8_t *cache, int j, int ids, uint4 (&r)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int blk = __shfl_sync(0xffffffffu, ids, i);
+                r[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the context, pages without a valid id
+                if (j < j1 && blk >= 0 && key_of(j) + 16 * i + row < ctx)
+                    r[i] = ldg_nc_v4(cache + (((size_t)blk * kKv8Page + row) * p.nkv + kvh) * kHD + 16 * ch);
+            }
+        };
+        // dims 16 ch ..: two 16-byte chunks of the half ch / 4.  The lanes of the second half write
+        // their odd chunk first, so that eight lanes cover all banks.
+        const int c0 = 2 * (ch & 3) + (ch >> 2), c1 = c0 ^ 1;
+        const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((c0 ^ (row & 7)) << 4);
+        const uint32_t dst1 = (ch >> 2) * kChHalf + row * 128 + ((c1 ^ (row & 7)) << 4);
+        auto convert = [&](uint32_t at, const uint4 (&r)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[2 * k] = e4m3x2_to_f16x2(w[k]), h[2 * k + 1] = e4m3x2hi_to_f16x2(w[k]);
+                const bool sw = ch >> 2;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 2048 + dst0),
+                             "r"(sw ? h[4] : h[0]), "r"(sw ? h[5] : h[1]), "r"(sw ? h[6] : h[2]), "r"(sw ? h[7] : h[3])
+                             : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 2048 + dst1),
+                             "r"(sw ? h[0] : h[4]), "r"(sw ? h[1] : h[5]), "r"(sw ? h[2] : h[6]), "r"(sw ? h[3] : h[7])
+                             : "memory");
+            }
+        };
+        auto publish = [&](uint64_t *m) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(m);
+        };
+        const uint32_t base = smem_u32(smem);
+        uint4 kr[8], vr[8];
+        int ids = fetch_ids(j0);
+        fetch(p.kc, j0, ids, kr);
+        fetch(p.vc, j0, ids, vr);
+        bool ok = true;
+        for (int j = j0, n = 0; j < j1 && ok; ++j, ++n) {
+            const int st = n & 1;
+            const uint32_t parity = (uint32_t)((n >> 1) - 1) & 1u;
+            // scales of the block's pages (warp 8: lanes 0..7 K, 8..15 V); zero without a valid id
+            float sc = 0.f;
+            if (warp == 8) {
+                const int blk = __shfl_sync(0xffffffffu, ids, lane & 7);
+                if (blk >= 0 && lane < 16) sc = (lane < 8 ? p.ks : p.vs)[(size_t)blk * p.nkv + kvh];
+            }
+            const int next = fetch_ids(j + 1);
+            if (n >= 2) ok = wait(&bar.k_empty[st], parity);
+            if (!ok) break;
+            if (warp == 8 && lane < 16) s_scale[n % kChScales][lane >> 3][lane & 7] = sc;
+            convert(base + (uint32_t)kChSmemK + st * kChOperand, kr);
+            publish(&bar.k_full[st]);
+            fetch(p.kc, j + 1, next, kr);
+            if (n >= 2) ok = wait(&bar.v_empty[st], parity);
+            if (!ok) break;
+            convert(base + (uint32_t)kChSmemV + st * kChOperand, vr);
+            publish(&bar.v_full[st]);
+            fetch(p.vc, j + 1, next, vr);
+            ids = next;
+        }
+    } else {
+        // ---- softmax: thread = row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const int rho = rho0 + t * kChTile + r;
+        const bool in = rho < rho1;
+        const size_t qrow = ((size_t)(q0 + (in ? rho / gsz : 0)) * p.nh + (size_t)kvh * gsz + (in ? rho % gsz : 0));
+        const int qp = in ? p0 + rho / gsz : -1;
+        float rowf;
+        {   // the row in f16 as q * 2^k, its largest magnitude in [2^14, 2^15), into the Q operand
+            uint4 w[16];
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                w[i] = in ? *reinterpret_cast<const uint4 *>(p.q + qrow * kHD + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t wd[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(wd[k] << 16)), fabsf(__uint_as_float(wd[k] & 0xffff0000u))));
+            }
+            int sh = 14 - ((int)(__float_as_uint(mx) >> 23) - 127);
+            sh = sh > 126 ? 126 : sh;
+            const float up = pow2f(sh);
+            rowf = pow2f(-sh) * kScoreScale;
+            const uint32_t dst = smem_u32(smem) + t * kChOperand + r * 128;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t wd[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                uint32_t h[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    h[k] = pack_f16(__uint_as_float(wd[k] << 16) * up, __uint_as_float(wd[k] & 0xffff0000u) * up);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i >> 3) * kChHalf +
+                                                                             (((i & 7) ^ (r & 7)) << 4)),
+                             "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3])
+                             : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.q_full);
+        }
+        float m = -INFINITY, l = 0.f, vref = 0.f, inv_vref = 0.f;
+        bool ok = true;
+        if (t < tiles) {
+            // positions of the warp's rows: blocks that all of them see whole need no mask
+            const int w0 = rho0 + t * kChTile + (warp & 3) * 32, w1 = min(rho1, w0 + 32) - 1;
+            const int pmin = p0 + w0 / gsz, pmax = p0 + (w1 >= w0 ? w1 : w0) / gsz;
+            const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * t, o_at = s_at + 256;
+            for (int j = j0, n = 0; j < j1; ++j, ++n) {
+                ok = wait(&bar.s_full[t], (uint32_t)n & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_ld32(s_at + 32 * c, s + 32 * c);
+                float f[8], c2[8];
+                {
+                    const float *sc = &s_scale[n % kChScales][0][0];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i];
+                }
+                float vtop = vref;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) vtop = fmaxf(vtop, c2[i]);
+                const int key0 = key_of(j);
+                const bool plain = key0 + kChKeys - 1 <= pmin &&
+                                   (p.geo.window == 0 || key0 > pmax - p.geo.window || key0 + kChKeys - 1 < p.geo.sinks);
+                tc_ld_wait();
+                if (!plain) {
+                    // scores scaled here (a factor of 0 must not meet an infinity), masked ones -inf
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) {
+                        const int key = key0 + i;
+                        const bool see = key <= qp && (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
+                        s[i] = __float_as_uint(see ? __uint_as_float(s[i]) * f[i >> 4] : -INFINITY);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = 1.f;
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float a = __uint_as_float(s[16 * i]), c = __uint_as_float(s[16 * i + 1]);
+#pragma unroll
+                    for (int k = 2; k < 16; k += 4) {
+                        a = max3(a, __uint_as_float(s[16 * i + k]), __uint_as_float(s[16 * i + k + 1]));
+                        if (k + 3 < 16) c = max3(c, __uint_as_float(s[16 * i + k + 2]), __uint_as_float(s[16 * i + k + 3]));
+                    }
+                    mx = fmaxf(mx, fmaxf(a, c) * f[i]);
+                }
+                // The fma below adds -m to an unrounded product: off by half a unit of m, which must
+                // stay far below 1.  Scores past 2^16 are rounded first, like m.
+                if (plain && __any_sync(0xffffffffu, fabsf(mx) > 65536.f)) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f[i >> 4]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = 1.f;
+                }
+                if (__any_sync(0xffffffffu, mx > m + kLag || vtop > vref)) {
+                    // s_full of this block came after the products of the last one: O is complete
+                    const float inv = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
+                    const float vfac = vref * inv, mn = fmaxf(m, mx);
+                    const float fm = mn == m ? 1.f : ex2(m - mn);
+                    vref = vtop, inv_vref = inv, m = mn;
+                    l *= fm;
+                    if (n > 0) {
+                        const float fo = fm * vfac;
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t u[16];
+                            asm volatile(
+                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+                                "%15}, [%16];"
+                                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+                                  "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+                                  "=r"(u[14]), "=r"(u[15])
+                                : "r"(o_at + 16 * c));
+                            tc_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * fo);
+                            asm volatile(
+                                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                                "%14,%15,%16};" ::"r"(o_at + 16 * c),
+                                "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+                                "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
+                                : "memory");
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : kProbBits - m;
+                // P over S: two scores per fma, the sum of a page's with its V scale taken out again
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float lr = fmaxf(lg2(c2[i] * inv_vref), -60.f);
+                    const uint64_t ff = f2_pack(f[i], f[i]), cc = f2_pack(base + lr, base + lr);
+                    uint64_t sum = 0ull;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint64_t e = f2_fma((uint64_t)s[16 * i + 2 * k] | ((uint64_t)s[16 * i + 2 * k + 1] << 32), ff, cc);
+                        float2 x = f2_unpack(e);
+                        x.x = ex2(x.x), x.y = ex2(x.y);
+                        sum = f2_add(sum, f2_pack(x.x, x.y));
+                        s[8 * i + k] = pack_f16(x.x, x.y);
+                    }
+                    const float2 y = f2_unpack(sum);
+                    l = fmaf(y.x + y.y, ex2(-lr), l);
+                    if (i == 3) tc_st32(s_at, s);
+                    if (i == 7) tc_st32(s_at + 32, s + 32);
+                }
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+            }
+            if (ok && j0 < j1) ok = wait(&bar.o_done, 0);
+            if (ok) {
+                tc_fence_after();
+                const float f = l > 0.f ? __fdiv_rn(vref, l) : 0.f;
+                const size_t ob = qrow * kHD;
+                float *rec = p.splits > 1 ? p.part + ((size_t)split * p.total_q * p.nh + qrow) * kRec : nullptr;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t u[32];
+                    __syncwarp();
+                    if (j0 < j1) {
+                        tc_ld32(o_at + 32 * c, u);
+                        tc_ld_wait();
+                    }
+                    if (!in) continue;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) u[k] = j0 < j1 ? __float_as_uint(__uint_as_float(u[k]) * f) : 0u;
+                    if (rec) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            *reinterpret_cast<uint4 *>(rec + 32 * c + 4 * k) =
+                                make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+                        continue;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float e[8];
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) e[x] = __uint_as_float(u[8 * k + x]);
+                        if (p.gate) apply_gate(e, p.gate + ob + 32 * c + 8 * k);
+                        store8(p.out + ob + 32 * c + 8 * k, e);
+                    }
+                }
+                if (rec && in) rec[kHD] = m, rec[kHD + 1] = l;
+            }
+        }
+    }
+    // ---- teardown ----
+    tc_fence_before();
+    __syncthreads();
+    if (s_abort && threadIdx.x == 0) atomicExch(&g_kv8_error, 1);
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Adds the splits of the chunk kernel.  A warp per (row, query head), lane l: dims 4l .. 4l + 3.
+__global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int num_seqs) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    // rows of the batch only: those behind the last sequence are not written
+    if (item >= (long long)p.geo.cu_q[num_seqs] * p.nh || item < (long long)p.geo.cu_q[0] * p.nh) return;
+    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float *rec = p.part + ((size_t)s * p.total_q * p.nh + item) * kRec;
+        const float m = rec[kHD], l = rec[kHD + 1];
+        const float4 o = *reinterpret_cast<const float4 *>(rec + 4 * lane);
+        const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2(M - mb), w = l * ex2(m - mb);
+        M = mn, L = L * f + w;
+        O[0] = O[0] * f + w * o.x, O[1] = O[1] * f + w * o.y, O[2] = O[2] * f + w * o.z, O[3] = O[3] * f + w * o.w;
+    }
+    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
+    finish4(p.out, p.gate, (size_t)item * kHD + 4 * lane, O, f);
 }
 
 // ---------------------------------------------------------------------------------
@@ -825,6 +1377,35 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
     return t;
 }
 
+struct ChunkPlan {
+    int rgs, splits;
+    size_t part_bytes;
+};
+
+// Calls of many rows per KV head run on the chunk kernel.  Its 128-row tiles cost the same however
+// few of their rows are used, and the token kernel's 16-row tiles each convert the cache anew.
+constexpr long long kChunkRows = 96;
+
+bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks, ChunkPlan &c) {
+    const int gsz = (int)(d->n_heads / d->n_kv_heads);
+    const long long max_q = (long long)(d->max_q_len < 1 ? 1 : (d->max_q_len < d->total_q ? d->max_q_len : d->total_q));
+    if (max_q * gsz < kChunkRows) return false;
+    c.rgs = (int)((max_q * gsz + kChRows - 1) / kChRows);
+    const long long ctas = (long long)d->num_seqs * c.rgs * (long long)d->n_kv_heads;
+    long long keys = (long long)d->max_context;
+    if (window > 0 && window < (1u << 30) && sinks < (1u << 30)) {
+        const long long seen = (long long)window + (long long)sinks + max_q + 2 * kChKeys;
+        if (seen < keys) keys = seen;
+    }
+    const long long blocks = (keys + kChKeys - 1) / kChKeys;
+    // fewer CTAs than SMs: split the keys, at least four blocks each
+    long long s = (num_sms() + ctas - 1) / ctas;
+    if (s > blocks / 4) s = blocks / 4;
+    c.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
+    c.part_bytes = c.splits > 1 ? (size_t)c.splits * d->total_q * d->n_heads * kRec * sizeof(float) : 0;
+    return ctas * c.splits <= 0x7fffffffLL;
+}
+
 int encode_pages(const uint8_t *kc, const uint8_t *vc, int nkv, int num_blocks, int hg, CUtensorMap (&maps)[2],
                  const char *what) {
     TensorMapEncodeTiledFn enc = tensor_map_encoder();
@@ -860,6 +1441,8 @@ extern "C" {
 size_t ekernel_paged_attention_kv8_workspace_bytes(const ekernel_paged_attn_desc_t *desc, size_t window,
                                                    size_t sinks) {
     if (kv8_check_desc(desc, "ekernel_paged_attention_kv8_workspace_bytes") != ECPU_OK) return 0;
+    ChunkPlan c;
+    if (plan_chunks(desc, window, sinks, c)) return c.part_bytes + 256;
     const TokPlan t = plan_tokens(desc, window, sinks);
     return t.part_bytes + t.prefix_bytes;
 }
@@ -878,10 +1461,48 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
     PILM_REQUIRE(!desc->output_gate || gate, ECPU_ERR_PARAM, "%s: gate required when output_gate", what);
     PILM_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out | (uintptr_t)gate) & 15) == 0,
                  ECPU_ERR_PARAM, "%s: the caches, q, gate and out must be 16-byte aligned", what);
-    const TokPlan t = plan_tokens(desc, window, sinks);
-    const size_t need = t.part_bytes + t.prefix_bytes;
+    const size_t need = ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks);
     PILM_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0, ECPU_ERR_PARAM,
                  "%s: workspace must be 16-byte aligned and hold %zu bytes, got %zu", what, need, workspace_bytes);
+    const size_t cap = 1u << 30;  // positions stay below it: a larger window is none
+    Geometry geo;
+    geo.cu_q = cu_q;
+    geo.ctx = context_lens;
+    geo.gsz = (int)(desc->n_heads / desc->n_kv_heads);
+    geo.window = window >= cap ? 0 : (int)window;
+    geo.sinks = (int)(sinks < cap ? sinks : cap);
+    ChunkPlan c;
+    if (plan_chunks(desc, window, sinks, c)) {
+        ChunkParams p;
+        p.geo = geo;
+        p.geo.rpg = kChRows;
+        p.geo.rgs = c.rgs;
+        p.q = (const __nv_bfloat16 *)q;
+        p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
+        p.kc = k_cache;
+        p.vc = v_cache;
+        p.ks = k_scale;
+        p.vs = v_scale;
+        p.block_table = block_table;
+        p.out = (__nv_bfloat16 *)out;
+        p.part = (float *)workspace;
+        p.nh = (int)desc->n_heads;
+        p.nkv = (int)desc->n_kv_heads;
+        p.max_blocks = (int)desc->max_blocks_per_seq;
+        p.num_blocks = (int)desc->num_blocks;
+        p.total_q = (int)desc->total_q;
+        p.splits = c.splits;
+        cudaFuncSetAttribute(kv8_attn_chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChSmem);
+        launch_pdl(kv8_attn_chunk, dim3((unsigned)(desc->num_seqs * c.rgs * c.splits), (unsigned)p.nkv), dim3(kChThreads),
+                   kChSmem, p);
+        rc = check_launch(what);
+        if (rc == ECPU_OK) rc = check_error(what);
+        if (rc != ECPU_OK || c.splits == 1) return rc;
+        const size_t items = desc->total_q * desc->n_heads;
+        launch_pdl(kv8_attn_join, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, p, (int)desc->num_seqs);
+        return check_launch(what);
+    }
+    const TokPlan t = plan_tokens(desc, window, sinks);
     CUtensorMap maps[2];
     rc = encode_pages(k_cache, v_cache, (int)desc->n_kv_heads, (int)desc->num_blocks, t.hg, maps, what);
     if (rc != ECPU_OK) return rc;
@@ -890,14 +1511,11 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         const int seqs = (int)(desc->num_seqs - b0 < (size_t)t.seqs_per_launch ? desc->num_seqs - b0
                                                                                : (size_t)t.seqs_per_launch);
         TokParams p;
-        p.geo.cu_q = cu_q + b0;
-        p.geo.ctx = context_lens + b0;
-        p.geo.gsz = (int)(desc->n_heads / desc->n_kv_heads);
+        p.geo = geo;
+        p.geo.cu_q += b0;
+        p.geo.ctx += b0;
         p.geo.rpg = t.rpg;
         p.geo.rgs = t.rgs;
-        const size_t cap = 1u << 30;  // positions stay below it: a larger window is none
-        p.geo.window = window >= cap ? 0 : (int)window;
-        p.geo.sinks = (int)(sinks < cap ? sinks : cap);
         p.q = (const __nv_bfloat16 *)q;
         p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
         p.ks = k_scale;
