@@ -874,6 +874,20 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // two floats at once
@@ -901,6 +915,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+// the largest of 16 floats
+__device__ __forceinline__ float max16(const uint32_t *s) {
+    float a = max3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
+    float b = max3(__uint_as_float(s[3]), __uint_as_float(s[4]), __uint_as_float(s[5]));
+    float c = max3(__uint_as_float(s[6]), __uint_as_float(s[7]), __uint_as_float(s[8]));
+    float d = max3(__uint_as_float(s[9]), __uint_as_float(s[10]), __uint_as_float(s[11]));
+    a = max3(a, __uint_as_float(s[12]), __uint_as_float(s[13]));
+    b = max3(b, __uint_as_float(s[14]), __uint_as_float(s[15]));
+    return fmaxf(max3(a, b, c), d);
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
@@ -1159,51 +1183,49 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                 ok = wait(&bar.s_full[t], (uint32_t)n & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tc_ld32(s_at + 32 * c, s + 32 * c);
-                float f[8], c2[8];
+                float f[8], c2[8], vtop = vref;
                 {
                     const float *sc = &s_scale[n % kChScales][0][0];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i];
+                    for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i], vtop = fmaxf(vtop, c2[i]);
                 }
-                float vtop = vref;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) vtop = fmaxf(vtop, c2[i]);
                 const int key0 = key_of(j);
-                const bool plain = key0 + kChKeys - 1 <= pmin &&
-                                   (p.geo.window == 0 || key0 > pmax - p.geo.window || key0 + kChKeys - 1 < p.geo.sinks);
-                tc_ld_wait();
-                if (!plain) {
-                    // scores scaled here (a factor of 0 must not meet an infinity), masked ones -inf
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) {
-                        const int key = key0 + i;
-                        const bool see = key <= qp && (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
-                        s[i] = __float_as_uint(see ? __uint_as_float(s[i]) * f[i >> 4] : -INFINITY);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = 1.f;
-                }
+                bool plain = key0 + kChKeys - 1 <= pmin &&
+                             (p.geo.window == 0 || key0 > pmax - p.geo.window || key0 + kChKeys - 1 < p.geo.sinks);
                 float mx = -INFINITY;
+                if (plain) {  // the maximum, page by page on the raw products
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float a = __uint_as_float(s[16 * i]), c = __uint_as_float(s[16 * i + 1]);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t s[64];
+                        tc_ld32(s_at + 64 * c, s);
+                        tc_ld32(s_at + 64 * c + 32, s + 32);
+                        tc_ld_wait();
 #pragma unroll
-                    for (int k = 2; k < 16; k += 4) {
-                        a = max3(a, __uint_as_float(s[16 * i + k]), __uint_as_float(s[16 * i + k + 1]));
-                        if (k + 3 < 16) c = max3(c, __uint_as_float(s[16 * i + k + 2]), __uint_as_float(s[16 * i + k + 3]));
+                        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, max16(s + 16 * i) * f[4 * c + i]);
                     }
-                    mx = fmaxf(mx, fmaxf(a, c) * f[i]);
+                    // The fma below adds -m to an unrounded product: off by half a unit of m, which
+                    // must stay far below 1.  Scores past 2^16 are rounded first, like m.
+                    plain = !__any_sync(0xffffffffu, fabsf(mx) > 65536.f);
                 }
-                // The fma below adds -m to an unrounded product: off by half a unit of m, which must
-                // stay far below 1.  Scores past 2^16 are rounded first, like m.
-                if (plain && __any_sync(0xffffffffu, fabsf(mx) > 65536.f)) {
+                if (!plain) {  // scaled scores (a factor of 0 must not meet an infinity), masked ones -inf
+                    mx = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f[i >> 4]);
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[32];
+                        tc_ld32(s_at + 32 * c, s);
+                        tc_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const int key = key0 + 32 * c + i;
+                            const bool see = key <= qp && (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
+                            s[i] = __float_as_uint(see ? __uint_as_float(s[i]) * f[2 * c + (i >> 4)] : -INFINITY);
+                        }
+                        mx = max3(mx, max16(s), max16(s + 16));
+                        tc_st32(s_at + 32 * c, s);
+                    }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = 1.f;
+                    tc_st_wait();
                 }
                 if (__any_sync(0xffffffffu, mx > m + kLag || vtop > vref)) {
                     // s_full of this block came after the products of the last one: O is complete
@@ -1217,44 +1239,39 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
 #pragma unroll 1
                         for (int c = 0; c < 8; ++c) {
                             uint32_t u[16];
-                            asm volatile(
-                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-                                "%15}, [%16];"
-                                : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
-                                  "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
-                                  "=r"(u[14]), "=r"(u[15])
-                                : "r"(o_at + 16 * c));
+                            tc_ld16(o_at + 16 * c, u);
                             tc_ld_wait();
 #pragma unroll
                             for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * fo);
-                            asm volatile(
-                                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-                                "%14,%15,%16};" ::"r"(o_at + 16 * c),
-                                "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
-                                "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-                                : "memory");
+                            tc_st16(o_at + 16 * c, u);
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : kProbBits - m;
-                // P over S: two scores per fma, the sum of a page's with its V scale taken out again
+                // P over S, 32 scores at a time (their 16 columns of P lie over columns read before):
+                // two scores per fma, the sum of a page's with its V scale taken out again
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float lr = fmaxf(lg2(c2[i] * inv_vref), -60.f);
-                    const uint64_t ff = f2_pack(f[i], f[i]), cc = f2_pack(base + lr, base + lr);
-                    uint64_t sum = 0ull;
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32], h[16];
+                    tc_ld32(s_at + 32 * c, s);
+                    tc_ld_wait();
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint64_t e = f2_fma((uint64_t)s[16 * i + 2 * k] | ((uint64_t)s[16 * i + 2 * k + 1] << 32), ff, cc);
-                        float2 x = f2_unpack(e);
-                        x.x = ex2(x.x), x.y = ex2(x.y);
-                        sum = f2_add(sum, f2_pack(x.x, x.y));
-                        s[8 * i + k] = pack_f16(x.x, x.y);
+                    for (int i = 0; i < 2; ++i) {
+                        const float lr = fmaxf(lg2(c2[2 * c + i] * inv_vref), -60.f);
+                        const uint64_t ff = f2_pack(f[2 * c + i], f[2 * c + i]), cc = f2_pack(base + lr, base + lr);
+                        uint64_t sum = 0ull;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint32_t *x2 = s + 16 * i + 2 * k;
+                            float2 x = f2_unpack(f2_fma((uint64_t)x2[0] | ((uint64_t)x2[1] << 32), ff, cc));
+                            x.x = ex2(x.x), x.y = ex2(x.y);
+                            sum = f2_add(sum, f2_pack(x.x, x.y));
+                            h[8 * i + k] = pack_f16(x.x, x.y);
+                        }
+                        const float2 y = f2_unpack(sum);
+                        l = fmaf(y.x + y.y, ex2(-lr), l);
                     }
-                    const float2 y = f2_unpack(sum);
-                    l = fmaf(y.x + y.y, ex2(-lr), l);
-                    if (i == 3) tc_st32(s_at, s);
-                    if (i == 7) tc_st32(s_at + 32, s + 32);
+                    tc_st16(s_at + 16 * c, h);
                 }
                 tc_st_wait();
                 tc_fence_before();
