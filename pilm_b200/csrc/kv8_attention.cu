@@ -1067,13 +1067,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             }
             return blk;
         };
-        auto fetch = [&](const uint8_t *cache, int j, int ids, uint4 (&r)[8]) {
+        // unconditional loads (of page 0 where there is none), so that all eight are in flight;
+        // what must not count is zeroed when it is converted
+        auto fetch = [&](const uint8_t *cache, int ids, uint4 (&r)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int blk = __shfl_sync(0xffffffffu, ids, i);
-                r[i] = make_uint4(0u, 0u, 0u, 0u);  // keys past the context, pages without a valid id
-                if (j < j1 && blk >= 0 && key_of(j) + 16 * i + row < ctx)
-                    r[i] = ldg_nc_v4(cache + (((size_t)blk * kKv8Page + row) * p.nkv + kvh) * kHD + 16 * ch);
+                const int blk = max(__shfl_sync(0xffffffffu, ids, i), 0);
+                r[i] = ldg_nc_v4(cache + (((size_t)blk * kKv8Page + row) * p.nkv + kvh) * kHD + 16 * ch);
             }
         };
         // dims 16 ch ..: two 16-byte chunks of the half ch / 4.  The lanes of the second half write
@@ -1081,10 +1081,12 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         const int c0 = 2 * (ch & 3) + (ch >> 2), c1 = c0 ^ 1;
         const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((c0 ^ (row & 7)) << 4);
         const uint32_t dst1 = (ch >> 2) * kChHalf + row * 128 + ((c1 ^ (row & 7)) << 4);
-        auto convert = [&](uint32_t at, const uint4 (&r)[8]) {
+        auto convert = [&](uint32_t at, int j, uint32_t valid, const uint4 (&r)[8]) {
+            const int keys = ctx - key_of(j) - row;  // keys past the context, pages without a valid id
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                const uint32_t on = ((valid >> i) & 1u) && 16 * i < keys ? ~0u : 0u;
+                const uint32_t w[4] = {r[i].x & on, r[i].y & on, r[i].z & on, r[i].w & on};
                 uint32_t h[8];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) h[2 * k] = e4m3x2_to_f16x2(w[k]), h[2 * k + 1] = e4m3x2hi_to_f16x2(w[k]);
@@ -1105,30 +1107,32 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         const uint32_t base = smem_u32(smem);
         uint4 kr[8], vr[8];
         int ids = fetch_ids(j0);
-        fetch(p.kc, j0, ids, kr);
-        fetch(p.vc, j0, ids, vr);
+        fetch(p.kc, ids, kr);
+        fetch(p.vc, ids, vr);
         bool ok = true;
         for (int j = j0, n = 0; j < j1 && ok; ++j, ++n) {
             const int st = n & 1;
             const uint32_t parity = (uint32_t)((n >> 1) - 1) & 1u;
             // scales of the block's pages (warp 8: lanes 0..7 K, 8..15 V); zero without a valid id
             float sc = 0.f;
+            const uint32_t valid = __ballot_sync(0xffffffffu, ids >= 0);
             if (warp == 8) {
                 const int blk = __shfl_sync(0xffffffffu, ids, lane & 7);
-                if (blk >= 0 && lane < 16) sc = (lane < 8 ? p.ks : p.vs)[(size_t)blk * p.nkv + kvh];
+                sc = (lane < 8 ? p.ks : p.vs)[(size_t)max(blk, 0) * p.nkv + kvh];
+                if (blk < 0) sc = 0.f;
             }
             const int next = fetch_ids(j + 1);
             if (n >= 2) ok = wait(&bar.k_empty[st], parity);
             if (!ok) break;
             if (warp == 8 && lane < 16) s_scale[n % kChScales][lane >> 3][lane & 7] = sc;
-            convert(base + (uint32_t)kChSmemK + st * kChOperand, kr);
+            convert(base + (uint32_t)kChSmemK + st * kChOperand, j, valid, kr);
             publish(&bar.k_full[st]);
-            fetch(p.kc, j + 1, next, kr);
+            fetch(p.kc, next, kr);
             if (n >= 2) ok = wait(&bar.v_empty[st], parity);
             if (!ok) break;
-            convert(base + (uint32_t)kChSmemV + st * kChOperand, vr);
+            convert(base + (uint32_t)kChSmemV + st * kChOperand, j, valid, vr);
             publish(&bar.v_full[st]);
-            fetch(p.vc, j + 1, next, vr);
+            fetch(p.vc, next, vr);
             ids = next;
         }
     } else {
