@@ -75,6 +75,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
+__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -832,26 +835,28 @@ __device__ __forceinline__ void tc_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
 }
-// SWIZZLE_128B operand, 1024 bytes between groups of 8 rows (of 8 keys, for the MN-major V), and
-// for V kChHalf between the two halves of the dims
-__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lead) {
-    return (uint64_t)((saddr & 0x3FFFF) >> 4) | ((uint64_t)lead << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// SWIZZLE_128B operand, 1024 bytes between groups of 8 rows (of 8 keys, for the MN-major V).  The
+// upper word of its descriptor is constant; the lower one holds the address / 16 and, for V, the
+// distance / 16 of the two halves of the dims.  An operand's next 16 columns (or keys) are an
+// addition to the lower word, so the issuing thread spends a few instructions per MMA.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t tc_desc(uint32_t saddr, uint32_t lead) { return ((saddr & 0x3FFFF) >> 4) | (lead << 16); }
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHi)
         : "memory");
 }
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t *r) {
@@ -933,7 +938,7 @@ __device__ __forceinline__ float lg2(float x) {
 }
 
 struct __align__(8) ChunkBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done;
 };
 
 // grid: (sequences x groups x splits, n_kv)
@@ -954,7 +959,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             mbar_init(&bar.v_full[i], 4);
             mbar_init(&bar.v_empty[i], 1);
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.p_full[i][0], 4);
+            mbar_init(&bar.p_full[i][1], 4);
         }
         mbar_init(&bar.o_done, 1);
         s_abort = 0;
@@ -972,9 +978,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     pdl_wait();
 
     // the last positions see the most keys: their groups first
-    const int split = blockIdx.x % p.splits, kvh = blockIdx.y;
-    const int seqs = (int)gridDim.x / (p.splits * p.geo.rgs);
-    const int gi = blockIdx.x / p.splits, b = gi % seqs, rg = p.geo.rgs - 1 - gi / seqs;
+    const int per = (int)gridDim.x / p.geo.rgs, rg = p.geo.rgs - 1 - blockIdx.x / per, in_rg = blockIdx.x % per;
+    const int split = in_rg % p.splits, kvh = in_rg / p.splits % p.nkv, b = in_rg / (p.splits * p.nkv);
     const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0, ctx = p.geo.ctx[b];
     const int gsz = p.geo.gsz, p0 = ctx - q_len;
     const int rho0 = rg * kChRows, rho1 = min(q_len * gsz, rho0 + kChRows);
@@ -1009,11 +1014,12 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             const uint32_t base = smem_u32(smem);
             auto issue_s = [&](int t, int n) {  // block n of this CTA
                 if (lane == 0) {
-                    const uint32_t qa = base + t * kChOperand, ka = base + (uint32_t)kChSmemK + (n & 1) * kChOperand;
+                    const uint32_t qa = tc_desc(base + t * kChOperand, 1);
+                    const uint32_t ka = tc_desc(base + (uint32_t)kChSmemK + (n & 1) * kChOperand, 1);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        tc_mma_ss(tmem + 128 * t, tc_desc(qa + (k >> 2) * kChHalf, 1) + 2 * (k & 3),
-                                  tc_desc(ka + (k >> 2) * kChHalf, 1) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
+                        tc_mma_ss(tmem + 128 * t, qa + (k >> 2) * (kChHalf >> 4) + 2 * (k & 3),
+                                  ka + (k >> 2) * (kChHalf >> 4) + 2 * (k & 3), idesc_s, k > 0 ? 1u : 0u);
                     tc_commit(&bar.s_full[t]);
                     if (t == tiles - 1) tc_commit(&bar.k_empty[n & 1]);
                 }
@@ -1028,15 +1034,26 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             for (int n = 0; ok && n < total; ++n) {
                 ok = wait(&bar.v_full[n & 1], (uint32_t)(n >> 1) & 1u);
                 for (int t = 0; ok && t < tiles; ++t) {
-                    ok = wait(&bar.p_full[t], (uint32_t)n & 1u);
+                    ok = wait(&bar.p_full[t][0], (uint32_t)n & 1u);
                     if (ok && n + 1 < total && t == 0) ok = wait(&bar.k_full[(n + 1) & 1], (uint32_t)((n + 1) >> 1) & 1u);
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        const uint32_t va = base + (uint32_t)kChSmemV + (n & 1) * kChOperand;
+                        const uint32_t va = tc_desc(base + (uint32_t)kChSmemV + (n & 1) * kChOperand, kChHalf >> 4);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)  // 16 keys: 8 columns of P, 16 rows of V
-                            tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, tc_desc(va + k * 2048, kChHalf >> 4),
+                        for (int k = 0; k < 4; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+                            tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, va + k * (2048 >> 4),
+                                      idesc_pv, n > 0 || k > 0 ? 1u : 0u);
+                    }
+                    __syncwarp();
+                    ok = wait(&bar.p_full[t][1], (uint32_t)n & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t va = tc_desc(base + (uint32_t)kChSmemV + (n & 1) * kChOperand, kChHalf >> 4);
+#pragma unroll
+                        for (int k = 4; k < 8; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+                            tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, va + k * (2048 >> 4),
                                       idesc_pv, n > 0 || k > 0 ? 1u : 0u);
                         if (t == tiles - 1) tc_commit(&bar.v_empty[n & 1]);
                     }
@@ -1082,21 +1099,18 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((c0 ^ (row & 7)) << 4);
         const uint32_t dst1 = (ch >> 2) * kChHalf + row * 128 + ((c1 ^ (row & 7)) << 4);
         auto convert = [&](uint32_t at, int j, uint32_t valid, const uint4 (&r)[8]) {
+            const bool whole = valid == 0xffu && key_of(j) + kChKeys <= ctx;
             const int keys = ctx - key_of(j) - row;  // keys past the context, pages without a valid id
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t on = ((valid >> i) & 1u) && 16 * i < keys ? ~0u : 0u;
-                const uint32_t w[4] = {r[i].x & on, r[i].y & on, r[i].z & on, r[i].w & on};
-                uint32_t h[8];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) h[2 * k] = e4m3x2_to_f16x2(w[k]), h[2 * k + 1] = e4m3x2hi_to_f16x2(w[k]);
-                const bool sw = ch >> 2;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 2048 + dst0),
-                             "r"(sw ? h[4] : h[0]), "r"(sw ? h[5] : h[1]), "r"(sw ? h[6] : h[2]), "r"(sw ? h[7] : h[3])
-                             : "memory");
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 2048 + dst1),
-                             "r"(sw ? h[0] : h[4]), "r"(sw ? h[1] : h[5]), "r"(sw ? h[2] : h[6]), "r"(sw ? h[3] : h[7])
-                             : "memory");
+                uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+                if (!whole && !(((valid >> i) & 1u) && 16 * i < keys)) w[0] = w[1] = w[2] = w[3] = 0u;
+                const bool sw = ch >> 2;  // the chunk written first: the second one's lanes swap the words
+                const uint32_t a0 = sw ? w[2] : w[0], a1 = sw ? w[3] : w[1], b0 = sw ? w[0] : w[2], b1 = sw ? w[1] : w[3];
+                const uint32_t x[4] = {e4m3x2_to_f16x2(a0), e4m3x2hi_to_f16x2(a0), e4m3x2_to_f16x2(a1), e4m3x2hi_to_f16x2(a1)};
+                const uint32_t y[4] = {e4m3x2_to_f16x2(b0), e4m3x2hi_to_f16x2(b0), e4m3x2_to_f16x2(b1), e4m3x2hi_to_f16x2(b1)};
+                sts128(at + i * 2048 + dst0, x);
+                sts128(at + i * 2048 + dst1, y);
             }
         };
         auto publish = [&](uint64_t *m) {
@@ -1276,11 +1290,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                         l = fmaf(y.x + y.y, ex2(-lr), l);
                     }
                     tc_st16(s_at + 16 * c, h);
+                    if (c & 1) {
+                        tc_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.p_full[t][c >> 1]);
+                    }
                 }
-                tc_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[t]);
             }
             if (ok && j0 < j1) ok = wait(&bar.o_done, 0);
             if (ok) {
@@ -1514,7 +1530,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.total_q = (int)desc->total_q;
         p.splits = c.splits;
         cudaFuncSetAttribute(kv8_attn_chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChSmem);
-        launch_pdl(kv8_attn_chunk, dim3((unsigned)(desc->num_seqs * c.rgs * c.splits), (unsigned)p.nkv), dim3(kChThreads),
+        launch_pdl(kv8_attn_chunk, dim3((unsigned)(desc->num_seqs * c.rgs * c.splits * p.nkv)), dim3(kChThreads),
                    kChSmem, p);
         rc = check_launch(what);
         if (rc == ECPU_OK) rc = check_error(what);
