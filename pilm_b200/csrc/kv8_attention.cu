@@ -175,12 +175,19 @@ __device__ __forceinline__ Group group_of(const Geometry &g, int vs) {
 }
 __device__ __forceinline__ int page_of(const Group &g, int v) { return v < g.n_sink ? v : v - g.n_sink + g.lo_page; }
 
-// CTA whose range [c*T/G, (c+1)*T/G) holds unit x
-__device__ __forceinline__ int cta_of(long long x, long long T, int G) {
-    int c = (int)((x * G) / T);
+// Shares of T units among G CTAs: CTA c has [share(c), share(c + 1)).  32-bit divisions where the
+// products fit (64-bit ones are subroutines, and took most of the merge kernel's time).
+__device__ __forceinline__ int share_of(int c, int T, int G) {
+    const unsigned long long n = (unsigned long long)c * (unsigned)T;
+    return (n >> 32) == 0 ? (int)((unsigned)n / (unsigned)G) : (int)(n / (unsigned)G);
+}
+// the CTA whose share holds unit x
+__device__ __forceinline__ int cta_of(int x, int T, int G) {
+    const unsigned long long n = (unsigned long long)x * (unsigned)G;
+    int c = (n >> 32) == 0 ? (int)((unsigned)n / (unsigned)T) : (int)(n / (unsigned)T);
     if (c >= G) c = G - 1;
-    while (c + 1 < G && ((long long)(c + 1) * T) / G <= x) ++c;
-    while (c > 0 && ((long long)c * T) / G > x) --c;
+    while (c + 1 < G && share_of(c + 1, T, G) <= x) ++c;
+    while (c > 0 && share_of(c, T, G) > x) --c;
     return c;
 }
 
@@ -222,6 +229,7 @@ struct TokParams {
     int *prefix_out;  // [groups + 1]: blocks before each group, for the merge
     int nh, nkv, max_blocks, num_blocks;
     int groups, hg, ch, kw, pps, stages, G;
+    int whole;  // a CTA per group (and head group) instead of equal shares of all pages
 };
 
 // Rows of a group that sees no key.
@@ -242,6 +250,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     __shared__ __align__(8) uint64_t full_bar[kTokStages], empty_bar[kTokStages], meet_bar;
     __shared__ float s_scale[kTokStages][2][16];  // [stage][K, V][page of the block * hg + head]
     __shared__ uint32_t s_valid[kTokStages];      // bit i: page i of the block has a valid id
+    __shared__ float2 s_ml[2][kTokWarps][16];     // [segment parity][warp][row]: max, sum
     __shared__ int s_abort;
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     pdl_trigger();
@@ -259,7 +268,20 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == kTokWarps && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &vmap : &kmap) : "memory");
     pdl_wait();
+    int x0, x1;  // this CTA's blocks
+    int v_first;       // the group of block x0
+    if (p.whole) {     // (s_prefix: only the CTA's own group, from 0)
+        const Group own = group_of(p.geo, cta);
+        v_first = cta;
+        x0 = 0, x1 = (own.nv + p.pps - 1) / p.pps;
+        __syncthreads();
+        if (x1 == 0) {
+            zero_rows(p, own, head0, p.hg);
+            return;
+        }
+    } else {
     if (warp == 0) {  // blocks before each group
         int carry = 0;
         if (lane == 0) s_prefix[0] = 0;
@@ -280,18 +302,17 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         for (int v = threadIdx.x; v <= p.groups; v += blockDim.x) p.prefix_out[v] = s_prefix[v];
     for (int v = cta; v < p.groups; v += p.G)
         if (s_prefix[v] == s_prefix[v + 1]) zero_rows(p, group_of(p.geo, v), head0, p.hg);
-    const long long T = s_prefix[p.groups];
-    const long long x0 = ((long long)cta * T) / p.G, x1 = ((long long)(cta + 1) * T) / p.G;
+    const int T = s_prefix[p.groups];
+    x0 = share_of(cta, T, p.G), x1 = share_of(cta + 1, T, p.G);
     if (x0 >= x1) return;
-    int v_first;  // the group of block x0
-    {
-        int lo = 0, hi = p.groups - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
-        }
-        v_first = lo;
+    int lo = 0, hi = p.groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
     }
+    v_first = lo;
+    }
+    auto start = [&](int v) { return p.whole ? (v == v_first ? 0 : x1) : s_prefix[v]; };
     const uint32_t ring = smem_u32(smem);
 
     if (warp >= kTokWarps) {
@@ -302,10 +323,10 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         Group g = group_of(p.geo, v);
         bool ok = true;
         // a block's page ids are fetched one block ahead (lane i: page i of the block)
-        auto fetch = [&](long long x, int &vv, Group &gg) {
+        auto fetch = [&](int x, int &vv, Group &gg) {
             if (x >= x1) return -1;
-            while (x >= s_prefix[vv + 1]) gg = group_of(p.geo, ++vv);
-            const int vp = (int)(x - s_prefix[vv]) * p.pps + lane;
+            while (x >= start(vv + 1)) gg = group_of(p.geo, ++vv);
+            const int vp = (x - start(vv)) * p.pps + lane;
             int blk = -1;
             if (lane < p.pps && vp < gg.nv) {
                 const int pg = page_of(gg, vp);
@@ -315,7 +336,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             return blk;
         };
         int next = fetch(x0, v, g);
-        for (long long x = x0; x < x1; ++x, ++issued) {
+        for (int x = x0; x < x1; ++x, ++issued) {
             const int blk = next;
             next = fetch(x + 1, v, g);
             const int st = issued % p.stages;
@@ -382,11 +403,12 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     int done = 0;  // blocks consumed
     int v = v_first;
     bool ok = true;
-    for (long long x = x0; x < x1 && ok;) {
-        while (x >= s_prefix[v + 1]) ++v;
+    int segs = 0;
+    for (int x = x0; x < x1 && ok; ++segs) {
+        while (x >= start(v + 1)) ++v;
         const Group g = group_of(p.geo, v);
-        const long long seg1 = min(x1, (long long)s_prefix[v + 1]);
-        const bool whole = x == s_prefix[v] && seg1 == s_prefix[v + 1];
+        const int seg1 = min(x1, start(v + 1));
+        const bool whole = x == start(v) && seg1 == start(v + 1);
         const int slot = x == x0 ? 0 : 1;
         const int tile0 = g.rho0 + 16 * c_of;
         const bool active = head_ok && tile0 < g.rho1;
@@ -455,7 +477,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                 ok = false;
                 break;
             }
-            const int vp = (int)(x - s_prefix[v]) * p.pps + 2 * k_of;
+            const int vp = (x - start(v)) * p.pps + 2 * k_of;
             if (active && vp < g.nv) {
                 const uint32_t kb = ring + st * stage_bytes + (2 * k_of) * page_bytes + h_of * 2048;
                 const uint32_t vb = kb + p.pps * page_bytes;
@@ -606,67 +628,61 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             for (int n = 0; n < 16; ++n) o[n][2 * hh] *= f, o[n][2 * hh + 1] *= f;
         }
         if (p.kw > 1) {
-            // The kw warps of each (head, tile) hold different pages' shares: warps 1.. hand theirs
-            // to warp 0, which adds them in order.  With one row tile the last stage's memory has
-            // room for all of them at once; else they go one by one through a buffer of their own.
+            // The kw warps of each (head, tile) hold different pages' shares.  They leave them in
+            // shared memory (the last stage's, which has room for one row tile; with more tiles in
+            // a buffer behind the ring) and each finishes every kw-th row.  16-byte chunk 8 c + i of
+            // a row lies at 8 c + (i ^ (c | (row & 1) << 2)): free of bank conflicts both ways.
             const int st = (done - 1) % p.stages;
-            const int at_once = p.ch == 1 ? p.kw - 1 : 1;
-            float *buf = reinterpret_cast<float *>(smem + (p.ch == 1 ? (size_t)st * stage_bytes
-                                                                     : (size_t)p.stages * stage_bytes)) +
-                         (size_t)(h_of * p.ch + c_of) * at_once * 16 * kRec;
+            float *buf = reinterpret_cast<float *>(smem + (size_t)(p.ch == 1 ? st : p.stages) * stage_bytes) +
+                         (size_t)(h_of * p.ch + c_of) * p.kw * 16 * kHD;
             ok = meet();  // every warp has read the stage
-            float w0[2] = {l[0], l[1]}, M[2] = {m[0], m[1]};
+            if (!ok) break;
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
+            for (int hh = 0; hh < 2; ++hh) {
+                const int r = g4 + 8 * hh;
+                float *row = buf + (k_of * 16 + r) * kHD;
 #pragma unroll
-                for (int n = 0; n < 16; ++n) o[n][2 * hh] *= w0[hh], o[n][2 * hh + 1] *= w0[hh];
-            for (int k0 = 1; k0 < p.kw && ok; k0 += at_once) {
-                if (k_of >= k0 && k_of < k0 + at_once) {
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        float *row = buf + (k_of - k0) * 16 * kRec + (g4 + 8 * hh) * kRec;
-#pragma unroll
-                        for (int n = 0; n < 16; ++n) {
-                            row[32 * c4 + n] = o[n][2 * hh];
-                            row[32 * c4 + 16 + n] = o[n][2 * hh + 1];
-                        }
-                        if (c4 == 0) row[kHD] = m[hh], row[kHD + 1] = l[hh];
+                for (int i = 0; i < 8; ++i) {
+                    const int e = 2 * hh + (i >> 2), n = 4 * (i & 3);
+                    *reinterpret_cast<float4 *>(row + 4 * (8 * c4 + (i ^ (c4 | (r & 1) << 2)))) =
+                        make_float4(o[n][e], o[n + 1][e], o[n + 2][e], o[n + 3][e]);
+                }
+                if (c4 == 0) s_ml[segs & 1][warp][r] = make_float2(m[hh], l[hh]);
+            }
+            ok = meet();
+            if (!ok) break;
+            if (active)
+                for (int r = k_of; r < tile1 - tile0; r += p.kw) {
+                    const float2 *ml = &s_ml[segs & 1][warp - k_of][r];
+                    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int k = 0; k < p.kw; ++k) M = fmaxf(M, ml[16 * k].x);
+                    const float Mb = M == -INFINITY ? 0.f : M;
+                    for (int k = 0; k < p.kw; ++k) {
+                        const float w = ml[16 * k].y * ex2(ml[16 * k].x - Mb);
+                        const float4 v = *reinterpret_cast<const float4 *>(
+                            buf + (k * 16 + r) * kHD + 4 * ((lane & 24) + ((lane & 7) ^ (lane >> 3 | (r & 1) << 2))));
+                        L += w;
+                        O[0] += w * v.x, O[1] += w * v.y, O[2] += w * v.z, O[3] += w * v.w;
+                    }
+                    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
+                    const int rho = tile0 + r;
+                    if (whole) {
+                        finish4(p.out, p.gate, ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD + 4 * lane, O, f);
+                    } else {
+                        float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.geo.rpg +
+                                               (size_t)h_of * p.geo.rpg + (rho - g.rho0)) * kRec;
+                        *reinterpret_cast<float4 *>(rec + 4 * lane) = make_float4(O[0] * f, O[1] * f, O[2] * f, O[3] * f);
+                        if (lane == 0) rec[kHD] = M, rec[kHD + 1] = L;
                     }
                 }
-                ok = meet();
-                if (k_of == 0 && ok) {
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-                        for (int k = 0; k < min(at_once, p.kw - k0); ++k) {
-                            const float *row = buf + k * 16 * kRec + (g4 + 8 * hh) * kRec;
-                            const float Mn = fmaxf(M[hh], row[kHD]), Mb = Mn == -INFINITY ? 0.f : Mn;
-                            const float f = ex2(M[hh] - Mb), w = ex2(row[kHD] - Mb);
-                            M[hh] = Mn;
-                            w0[hh] = w0[hh] * f + row[kHD + 1] * w;
-#pragma unroll
-                            for (int n = 0; n < 16; ++n) {
-                                o[n][2 * hh] = o[n][2 * hh] * f + w * row[32 * c4 + n];
-                                o[n][2 * hh + 1] = o[n][2 * hh + 1] * f + w * row[32 * c4 + 16 + n];
-                            }
-                        }
-                }
-                if (at_once == 1) ok = meet() && ok;  // before the buffer's next use
-            }
-            if (!ok) break;
-            if (k_of == 0)
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    const float f = w0[hh] > 0.f ? __fdiv_rn(1.f, w0[hh]) : 0.f;
-#pragma unroll
-                    for (int n = 0; n < 16; ++n) o[n][2 * hh] *= f, o[n][2 * hh + 1] *= f;
-                    m[hh] = M[hh], l[hh] = w0[hh];
-                }
-            // writes here come before the copies into this stage
+            if (p.ch > 1) ok = meet();  // before the buffer's next use
+            // reads and writes here come before the copies into this stage
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[st]);
+            continue;
         }
-        if (!active || k_of > 0) continue;
+        if (!active) continue;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
             const int rho = tile0 + g4 + 8 * hh;
@@ -716,7 +732,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokPara
     const bool in = head < p.nh && j < q_len;
     const int kvh = in ? head / p.geo.gsz : 0, rho = j * p.geo.gsz + (in ? head % p.geo.gsz : 0);
     const int v = b * p.geo.rgs + rho / p.geo.rpg;
-    const long long T = p.prefix_out[p.groups], P0 = in ? p.prefix_out[v] : 0, P1 = in ? p.prefix_out[v + 1] : 0;
+    const int T = p.prefix_out[p.groups], P0 = in ? p.prefix_out[v] : 0, P1 = in ? p.prefix_out[v + 1] : 0;
     int c0 = 0, c1 = -1;
     if (P1 > P0) {
         const int c = cta_of(lane == 0 ? P0 : P1 - 1, T, p.G);
@@ -736,7 +752,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokPara
             // fills its beginning), or none where its range is empty
             int sl = -1;
             if (lane < U && cb + lane <= c1) {
-                const long long lo = ((long long)(cb + lane) * T) / p.G, hi = ((long long)(cb + lane + 1) * T) / p.G;
+                const int lo = share_of(cb + lane, T, p.G), hi = share_of(cb + lane + 1, T, p.G);
                 if (hi > lo) sl = lo >= P0 ? 0 : 1;
             }
 #pragma unroll
@@ -1372,7 +1388,7 @@ __global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int nu
 // Host side
 // ---------------------------------------------------------------------------------
 struct TokPlan {
-    int hg, ngroups, ch, kw, pps, rpg, rgs, G, stages, seqs_per_launch;
+    int hg, ngroups, ch, kw, pps, rpg, rgs, G, whole, stages, seqs_per_launch;
     size_t stage_bytes, smem, part_bytes, prefix_bytes;
 };
 
@@ -1380,36 +1396,53 @@ constexpr size_t kTokSmem = 200 * 1024;  // ring; with the static arrays below t
 
 TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks) {
     TokPlan t;
-    const int nkv = (int)d->n_kv_heads, gsz = (int)(d->n_heads / d->n_kv_heads);
+    const int nkv = (int)d->n_kv_heads, gsz = (int)(d->n_heads / d->n_kv_heads), sms = num_sms();
     const long long max_q = (long long)(d->max_q_len < 1 ? 1 : (d->max_q_len < d->total_q ? d->max_q_len : d->total_q));
     const long long rows = max_q * gsz;
-    // row tiles first (they share the pages a CTA reads), then as many KV heads as fill the warps
-    t.ch = (int)(rows > 16 * kTokWarps ? kTokWarps : (rows + 15) / 16);
-    const int most = kTokWarps / t.ch;
-    t.ngroups = (nkv + most - 1) / most;
-    t.hg = (nkv + t.ngroups - 1) / t.ngroups;
-    t.kw = kTokWarps / (t.hg * t.ch);
-    t.pps = 2 * t.kw;
+    t.ch = (int)(rows > 16 * kTokWarps ? kTokWarps : (rows + 15) / 16);  // row tiles share the pages a CTA reads
     t.rpg = 16 * t.ch;
     t.rgs = (int)((rows + t.rpg - 1) / t.rpg);
+    long long keys = (long long)d->max_context;
+    if (window > 0 && window < (1u << 30) && sinks < (1u << 30)) {
+        const long long seen = (long long)window + (long long)sinks + max_q + 32;
+        if (seen < keys) keys = seen;
+    }
+    const long long pages = (keys + 15) / 16, groups = (long long)d->num_seqs * t.rgs;
+    auto shape = [&](int heads) {  // KV heads per CTA, the rest of the warps on different pages
+        t.ngroups = (nkv + heads - 1) / heads;
+        t.hg = (nkv + t.ngroups - 1) / t.ngroups;
+        t.kw = kTokWarps / (t.hg * t.ch);
+        t.pps = 2 * t.kw;
+    };
+    // Equal shares of all pages: as many KV heads per CTA as fill the warps (long contiguous reads),
+    // one CTA per SM over the head groups, at least one block of pages each.
+    shape(kTokWarps / t.ch);
+    const long long per = sms / t.ngroups < 1 ? 1 : sms / t.ngroups;
+    const long long blocks = groups * ((pages + t.pps - 1) / t.pps);
+    t.whole = 0;
+    t.G = (int)(blocks < 1 ? 1 : (blocks < per ? blocks : per));
+    const long long share = (blocks + t.G - 1) / t.G;
+    // Or a CTA for each group and as few heads as the SMs allow: no partials, no second launch, whose
+    // time is that of about four blocks (measured: 3 us, 0.8 us a block).
+    for (int heads = 1; heads <= kTokWarps / t.ch; heads *= 2) {
+        if (groups * ((nkv + heads - 1) / heads) > sms) continue;
+        const TokPlan shares = t;
+        shape(heads);
+        if ((pages + t.pps - 1) / t.pps <= share + 4) {
+            t.whole = 1;
+            t.G = (int)groups;
+        } else {
+            t = shares;
+        }
+        break;
+    }
     t.seqs_per_launch = t.rgs >= kTokGroups ? 1 : kTokGroups / t.rgs;
     t.stage_bytes = (size_t)t.pps * t.hg * 4096;
-    const size_t join = t.kw > 1 && t.ch > 1 ? (size_t)t.hg * t.ch * 16 * kRec * sizeof(float) : 0;
+    const size_t join = t.kw > 1 && t.ch > 1 ? (size_t)t.hg * t.ch * t.kw * 16 * kHD * sizeof(float) : 0;
     t.stages = (int)((kTokSmem - join) / t.stage_bytes);
     if (t.stages > kTokStages) t.stages = kTokStages;
     t.smem = t.stages * t.stage_bytes + join + 1024;
-    // one CTA per SM over the head groups, but no more than leaves each a few blocks by the
-    // host's bound on the batch's pages
-    long long keys = (long long)d->max_context;
-    if (window > 0) {
-        const long long seen = (long long)window + (long long)sinks + max_q + 32;
-        if (seen < keys && window < (1u << 30) && sinks < (1u << 30)) keys = seen;
-    }
-    const long long blocks = (long long)d->num_seqs * t.rgs * ((keys + 16 * t.pps - 1) / (16 * t.pps));
-    const int per = num_sms() / t.ngroups < 1 ? 1 : num_sms() / t.ngroups;
-    const long long want = (blocks + 3) / 4;
-    t.G = (int)(want < 1 ? 1 : (want < per ? want : per));
-    t.part_bytes = (size_t)t.ngroups * t.G * 2 * t.hg * t.rpg * kRec * sizeof(float);
+    t.part_bytes = t.whole ? 0 : (size_t)t.ngroups * t.G * 2 * t.hg * t.rpg * kRec * sizeof(float);
     t.prefix_bytes = (size_t)(kTokGroups + 4) * sizeof(int);
     return t;
 }
@@ -1572,13 +1605,14 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.pps = t.pps;
         p.stages = t.stages;
         p.G = t.G;
+        p.whole = t.whole;
         launch_pdl(kv8_attn_tokens, dim3((unsigned)t.G, (unsigned)t.ngroups), dim3(kTokThreads), t.smem,
                    maps[0], maps[1], p);
         rc = check_launch(what);
         if (rc != ECPU_OK) return rc;
         rc = check_error(what);
         if (rc != ECPU_OK) return rc;
-        if (t.G == 1) continue;  // every group whole
+        if (t.G == 1 || t.whole) continue;  // every group whole
         // a row of the batch is the longest a sequence can have
         const int max_q = (int)(desc->max_q_len < 1 ? 1 : (desc->max_q_len < desc->total_q ? desc->max_q_len : desc->total_q));
         const int wpi = t.G > 16 * seqs * t.rgs ? kMergeWarps : 1;
