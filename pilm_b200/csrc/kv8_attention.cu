@@ -217,6 +217,7 @@ constexpr int kTokWarps = 8;      // consumer warps at most
 constexpr int kTokThreads = 384;
 constexpr int kTokGroups = 4096;  // groups per launch (their prefix is kept in shared memory)
 constexpr int kTokStages = 8;     // ring stages at most
+constexpr int kMergeScan = 128;   // groups up to which the merge works out the prefix itself
 constexpr int kRec = kHD + 4;     // a partial: O[128] normalised, max (base 2), sum, two pad floats
 
 struct TokParams {
@@ -253,7 +254,6 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     __shared__ float2 s_ml[2][kTokWarps][16];     // [segment parity][warp][row]: max, sum
     __shared__ int s_abort;
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int consumers = p.hg * p.ch * p.kw;
     const int cta = blockIdx.x, head0 = blockIdx.y * p.hg;
@@ -270,6 +270,9 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     }
     if (warp == kTokWarps && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &vmap : &kmap) : "memory");
     pdl_wait();
+    // only now: the merge kernel reads the batch's geometry before it waits for this one, and what
+    // came before this one (which may have written it) is complete here
+    pdl_trigger();
     int x0, x1;  // this CTA's blocks
     int v_first;       // the group of block x0
     if (p.whole) {     // (s_prefix: only the CTA's own group, from 0)
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         }
     }
     __syncthreads();
-    if (cta == 0 && blockIdx.y == 0 && p.prefix_out)
+    if (cta == 0 && blockIdx.y == 0 && p.groups > kMergeScan)
         for (int v = threadIdx.x; v <= p.groups; v += blockDim.x) p.prefix_out[v] = s_prefix[v];
     for (int v = cta; v < p.groups; v += p.G)
         if (s_prefix[v] == s_prefix[v + 1]) zero_rows(p, group_of(p.geo, v), head0, p.hg);
@@ -716,33 +719,45 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     }
 }
 
-// Combines the partials that CTA range boundaries cut.  A block takes one (row, query head), or
-// blockDim / (32 * wpi) of them; wpi warps share one's partials (many CTAs on one sequence), each
-// 8 in flight, and join through shared memory.  Lane l takes dims 4l .. 4l + 3.
-constexpr int kMergeWarps = 8;
-__global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokParams p, int wpi) {
-    __shared__ float s_o[kMergeWarps][kHD], s_ml[kMergeWarps][2];
+// Combines the partials that CTA range boundaries cut.  A block's WPB warps take one (row, query
+// head) each, or wpi of them share one's partials (many CTAs on one sequence) and join through
+// shared memory; U partials in flight per warp, lane l takes dims 4l .. 4l + 3.  The shares follow
+// from the contexts, which the token kernel only reads: for up to kMergeScan groups they are worked
+// out before the wait for it, and one round of loads remains.
+template <int WPB, int U>
+__global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, int wpi) {
+    __shared__ float s_o[WPB][kHD], s_ml[WPB][2];
     pdl_trigger();
-    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % wpi;
-    const int per = kMergeWarps / wpi, hb = (p.nh + per - 1) / per;
+    const int per = WPB / wpi, hb = (p.nh + per - 1) / per;
     const int head = blockIdx.x % hb * per + warp / wpi;
     const int j = blockIdx.x / hb, b = blockIdx.y;
     const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0;
     const bool in = head < p.nh && j < q_len;
     const int kvh = in ? head / p.geo.gsz : 0, rho = j * p.geo.gsz + (in ? head % p.geo.gsz : 0);
     const int v = b * p.geo.rgs + rho / p.geo.rpg;
-    const int T = p.prefix_out[p.groups], P0 = in ? p.prefix_out[v] : 0, P1 = in ? p.prefix_out[v + 1] : 0;
+    int T = 0, P0 = 0, P1 = 0;
+    if (p.groups <= kMergeScan) {
+        for (int v0 = 0; v0 < p.groups; v0 += 32) {
+            const int x = v0 + lane, n = x < p.groups ? (group_of(p.geo, x).nv + p.pps - 1) / p.pps : 0;
+            T += __reduce_add_sync(0xffffffffu, n);
+            P0 += __reduce_add_sync(0xffffffffu, x < v ? n : 0);
+            P1 += __reduce_add_sync(0xffffffffu, x <= v ? n : 0);
+        }
+    } else {
+        pdl_wait();
+        T = p.prefix_out[p.groups], P0 = p.prefix_out[v], P1 = p.prefix_out[v + 1];
+    }
     int c0 = 0, c1 = -1;
-    if (P1 > P0) {
+    if (in && P1 > P0) {
         const int c = cta_of(lane == 0 ? P0 : P1 - 1, T, p.G);
         c0 = __shfl_sync(0xffffffffu, c, 0), c1 = __shfl_sync(0xffffffffu, c, 1);
     }
+    pdl_wait();
     const bool cut = c1 > c0;  // else its one CTA wrote the output
     const size_t rows = (size_t)p.hg * p.geo.rpg;
     const float *base = p.part + ((size_t)(kvh / p.hg) * p.G * 2) * rows * kRec +
                         ((size_t)(kvh % p.hg) * p.geo.rpg + rho % p.geo.rpg) * kRec;
-    constexpr int U = 8;
     float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
     if (cut)
         for (int cb = c0 + sub * U; cb <= c1; cb += wpi * U) {
@@ -755,17 +770,20 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv8_attn_merge(const TokPara
                 const int lo = share_of(cb + lane, T, p.G), hi = share_of(cb + lane + 1, T, p.G);
                 if (hi > lo) sl = lo >= P0 ? 0 : 1;
             }
+            // unconditional loads (of the group's first partial where there is none): all in flight
+            float4 ml[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int slot = __shfl_sync(0xffffffffu, sl, u);
-                m[u] = -INFINITY, l[u] = 0.f;
-                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (slot >= 0) {
-                    const float *rec = base + ((size_t)(cb + u) * 2 + slot) * rows * kRec;
-                    m[u] = __ldcg(rec + kHD);
-                    l[u] = __ldcg(rec + kHD + 1);
-                    o[u] = __ldcg(reinterpret_cast<const float4 *>(rec + 4 * lane));
-                }
+                const float *rec = base + ((size_t)(slot < 0 ? c0 : cb + u) * 2 + max(slot, 0)) * rows * kRec;
+                ml[u] = __ldcg(reinterpret_cast<const float4 *>(rec + kHD));
+                o[u] = __ldcg(reinterpret_cast<const float4 *>(rec + 4 * lane));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool none = __shfl_sync(0xffffffffu, sl, u) < 0;
+                m[u] = none ? -INFINITY : ml[u].x, l[u] = none ? 0.f : ml[u].y;
+                if (none) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float mc = M;
 #pragma unroll
@@ -1615,10 +1633,12 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         if (t.G == 1 || t.whole) continue;  // every group whole
         // a row of the batch is the longest a sequence can have
         const int max_q = (int)(desc->max_q_len < 1 ? 1 : (desc->max_q_len < desc->total_q ? desc->max_q_len : desc->total_q));
-        const int wpi = t.G > 16 * seqs * t.rgs ? kMergeWarps : 1;
-        const int per = kMergeWarps / wpi;
-        launch_pdl(kv8_attn_merge, dim3((unsigned)((p.nh + per - 1) / per * max_q), (unsigned)seqs),
-                   dim3(kMergeWarps * 32), 0, p, wpi);
+        // few groups over many CTAs: all of a block's warps on one row and head's partials
+        const bool wide = t.G > 16 * seqs * t.rgs;
+        const int per = wide ? 1 : 8;
+        launch_pdl(wide ? kv8_attn_merge<16, 10> : kv8_attn_merge<8, 8>,
+                   dim3((unsigned)((p.nh + per - 1) / per * max_q), (unsigned)seqs), dim3(wide ? 512 : 256), 0, p,
+                   wide ? 16 : 1);
         rc = check_launch(what);
         if (rc != ECPU_OK) return rc;
     }
