@@ -202,7 +202,8 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
 
     from pilm_b200 import bindings
     from pilm_b200.engine import MTPVerifyEngine
-    from pilm_b200.qwen3 import QWEN3_8B, PagedKVCache, Qwen3Verifier, Qwen3Weights, attention_bytes
+    from pilm_b200.qwen3 import (QWEN3_8B, PagedKVCache, PagedKVCacheKV8, Qwen3Verifier, Qwen3Weights,
+                                 attention_bytes)
 
     torch.cuda.set_device(local_rank)
     dev = torch.device("cuda", local_rank)
@@ -216,9 +217,11 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
     weights = Qwen3Weights.synthetic(shape, seed, dev)
     pages_per_seq = (PROMPT + GEN_HEADROOM + PAGE - 1) // PAGE
     num_blocks = SEQS * pages_per_seq + 1
-    kv = PagedKVCache(shape, num_blocks, dev, fill="random", seed=seed)
+    kv8 = args.kv == "e4m3"
+    kv = (PagedKVCacheKV8 if kv8 else PagedKVCache)(shape, num_blocks, dev, fill="random", seed=seed)
     max_rows = SEQS * (K_DRAFT + 1)
-    ver = Qwen3Verifier(weights, kv, max_rows=max_rows, max_pos=PROMPT + GEN_HEADROOM + 64, device=dev)
+    ver = Qwen3Verifier(weights, kv, max_rows=max_rows, max_pos=PROMPT + GEN_HEADROOM + 64, device=dev,
+                        window=args.window, sinks=args.sinks)
     eng = MTPVerifyEngine(ver, num_blocks=num_blocks, max_model_len=PROMPT + GEN_HEADROOM + 64)
     g = torch.Generator().manual_seed(seed)
     for _ in range(SEQS):
@@ -416,7 +419,9 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
     # ---- roofline of the dominant kernel (paged attention) -------------------------
     pk = peaks()
     ctx = batch.context_lens.tolist()
-    att_bytes = attention_bytes(shape, ctx, [1 + K_DRAFT] * SEQS)
+    if args.window:
+        ctx = [min(c, args.window + K_DRAFT + args.sinks) for c in ctx]
+    att_bytes = attention_bytes(shape, ctx, [1 + K_DRAFT] * SEQS, 1 if kv8 else 2)
     att_ms = op_ms.get("attention")
     att_gbs = att_bytes / (att_ms * 1e-3) / 1e9 if att_ms else None
     lin_bytes = weights.linear_bytes
@@ -428,7 +433,7 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
     # grows (it reads each K/V byte once)
     kv_bytes = sum(ctx) * shape.n_kv_heads * shape.head_dim * 2 * 2
     cap = attn_traffic_capture()
-    traffic = round(cap["bytes"] * kv_bytes / cap["kv_bytes"]) if cap else None
+    traffic = round(cap["bytes"] * kv_bytes / cap["kv_bytes"]) if cap and not kv8 else None
     # the CPU baseline runs at N = 1 only: at N > 1 the host's cores serve every rank
     cpu = cpu_baseline_sample(args) if not args.no_cpu and world == 1 else None
     value = rows_per_step * world / (ms_max * 1e-3)
@@ -445,7 +450,8 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
         "vs_baseline": None,
         "dtype": "bf16 activations x int4 weights, fp32 accumulate",
         "data": "synthetic (seeded random-init weights, random prompt KV pages, random drafts)",
-        "config": bench_config(shape.layers, world, SEQS, PROMPT),
+        "config": dict(bench_config(shape.layers, world, SEQS, PROMPT),
+                       **({"kv_cache": "e4m3", "window": args.window, "sinks": args.sinks} if kv8 else {})),
         "per_gpu": round(value / world, 2),
         "e2e": {
             "value": round(e2e_rows_all / max(1, e2e_steps) / (e2e_ms_max * 1e-3), 2) if e2e_steps else None,
@@ -460,7 +466,8 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
         "cycle_bf16_drafter": cycle_bf16,
         "e2e_accepting": accepting,
         "roofline": {
-            "kernel": "attn_pages (+ attn_merge_pages), per layer",
+            "kernel": "kv8_attn_tokens (+ kv8_attn_merge), per layer" if kv8 else
+                      "attn_pages (+ attn_merge_pages), per layer",
             "bound": "hbm",
             "achieved": round(att_gbs, 1) if att_gbs else None,
             "peak": pk["hbm_gbs"],
@@ -1186,6 +1193,11 @@ def main():
                     help="skip the leg whose drafts are accepted (the model's own greedy continuation)")
     ap.add_argument("--seqs", type=int, default=SEQS, help="sequences per GPU (default: the BASELINE config)")
     ap.add_argument("--prompt", type=int, default=PROMPT, help="prompt tokens per sequence")
+    ap.add_argument("--kv", default="bf16", choices=["bf16", "e4m3"],
+                    help="KV cache of the bench line: bf16 (the default workload) or 8-bit e4m3 codes with a scale "
+                         "per page and KV head")
+    ap.add_argument("--window", type=int, default=0, help="with --kv e4m3: sliding attention window (0: none)")
+    ap.add_argument("--sinks", type=int, default=0, help="with --window: first tokens that stay visible")
     ap.add_argument("--layers", type=int, default=0, help="decoder layers (0 = all 36); profiling only")
     ap.add_argument("--sweep", default=None,
                     help="per-kernel op sweep instead of the bench line: all, or any of linear,attention,accept")

@@ -252,6 +252,43 @@ class PagedKVCache:
         return len(self.k) * 2 * self.k[0].shape[2] * self.k[0].shape[3] * self.k[0].element_size()
 
 
+class PagedKVCacheKV8:
+    """Device-resident paged KV in 8 bits: per layer K and V e4m3 codes (uint8
+    [num_blocks, block_size, n_kv, hd]) and one fp32 scale for each page and KV head
+    ([num_blocks, n_kv]).  Half the bytes of PagedKVCache; pages and slots mean the same.
+    Codes start as zeros with scales of 1."""
+
+    def __init__(self, shape: Qwen3Shape, num_blocks: int, device, fill: Optional[str] = None, seed: int = 0):
+        """fill="random": the values PagedKVCache's random fill draws, quantized page by page as
+        the append quantizes them."""
+        if shape.head_dim != 128 or shape.block_size != 16:
+            raise ValueError("the 8-bit KV cache takes head_dim 128 and 16-token pages")
+        self.num_blocks = num_blocks
+        self.block_size = shape.block_size
+        self.dtype = torch.float8_e4m3fn
+        dims = (num_blocks, shape.block_size, shape.n_kv_heads, shape.head_dim)
+        g = torch.Generator(device=device).manual_seed(seed) if fill == "random" else None
+        self.k, self.v, self.k_scale, self.v_scale = [], [], [], []
+        for _ in range(shape.layers):
+            for codes, scales, std in ((self.k, self.k_scale, 1.0), (self.v, self.v_scale, 0.02)):
+                scale = torch.ones((num_blocks, shape.n_kv_heads), dtype=torch.float32, device=device)
+                if g is None:
+                    code = torch.zeros(dims, dtype=torch.uint8, device=device)
+                else:
+                    x = torch.randn(dims, generator=g, device=device, dtype=torch.float32).mul_(std).to(torch.bfloat16)
+                    m, e = torch.frexp(x.abs().amax((1, 3)).float())   # 448 = 0.875 * 2^9
+                    scale = torch.ldexp(scale, e - 9 + (m > 0.875))
+                    code = (x.float() / scale[:, None, :, None]).to(torch.float8_e4m3fn).view(torch.uint8)
+                codes.append(code)
+                scales.append(scale)
+
+    @property
+    def bytes_per_token(self) -> int:
+        """Codes and the token's share of its page's scales, rounded up."""
+        layers, kv, hd = len(self.k), self.k[0].shape[2], self.k[0].shape[3]
+        return layers * 2 * kv * hd + -(-layers * 2 * kv * 4 // self.block_size)
+
+
 @dataclass
 class VerifyBatch:
     """Device metadata of one verify (or prefill-chunk) pass over B sequences."""
@@ -299,10 +336,22 @@ def attention_slices(cu_q, context_lens, group: int, max_slices: int = 1024):
 class Qwen3Verifier:
     """Runs the batched verify forward, the LM head and the acceptance kernels."""
 
-    def __init__(self, weights: Qwen3Weights, kv: PagedKVCache, max_rows: int, max_pos: int, device):
+    def __init__(self, weights: Qwen3Weights, kv: "PagedKVCache | PagedKVCacheKV8", max_rows: int, max_pos: int, device,
+                 window: int = 0, sinks: int = 0):
+        """kv: the bf16 cache, or the 8-bit one (PagedKVCacheKV8).  window > 0, on the 8-bit cache:
+        every layer's attention sees the last `window` positions and the first `sinks`."""
         self.w = weights
         self.shape = weights.shape
         self.kv = kv
+        self.kv8 = isinstance(kv, PagedKVCacheKV8)
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        if window and not self.kv8:
+            raise ValueError("attention through a sliding window runs on the 8-bit KV cache (PagedKVCacheKV8)")
+        self.window, self.sinks = int(window), int(sinks)
+        # workspaces of the 8-bit cache attention; an outgrown one is kept, since graphs captured
+        # while it was current replay into it
+        self._kv8_ws: list[torch.Tensor] = []
         self.device = device
         self.max_rows = max_rows
         s = self.shape
@@ -405,7 +454,7 @@ class Qwen3Verifier:
         cu_q, which a replay with other row counts would not update."""
         s = self.shape
         gsz = s.n_heads // s.n_kv_heads
-        if (not self.slice_attention or b.max_q_len * gsz <= 16 or gsz > 16
+        if (self.kv8 or not self.slice_attention or b.max_q_len * gsz <= 16 or gsz > 16
                 or torch.cuda.is_current_stream_capturing()):
             return None
         cut = attention_slices(b.cu_q.cpu().numpy(), b.context_lens.cpu().numpy(), gsz)
@@ -419,6 +468,37 @@ class Qwen3Verifier:
                          max_context=int(ctx_v.max()))
         return self._desc(vb), vb
 
+    def _kv8_workspace(self, desc) -> torch.Tensor:
+        n = ck.paged_attention_kv8_workspace_bytes(desc, self.window, self.sinks)
+        if not self._kv8_ws or self._kv8_ws[-1].numel() < n:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the attention workspace cannot grow during capture: run the shape once before")
+            self._kv8_ws.append(torch.empty(n, dtype=torch.uint8, device=self.device))
+        return self._kv8_ws[-1]
+
+    def _append(self, desc, li: int, L: dict, b: VerifyBatch, part, splits: int) -> None:
+        """QK-norm, RoPE and the layer's KV append, from the projection or its split-K partials."""
+        T, kv = b.total_q, self.kv
+        gate = self.gate[:T] if self.shape.gated else None
+        head = (part, splits) if splits else (self.qkv[:T],)
+        tail = (L["q_norm"], L["k_norm"], self.cos, self.sin, b.positions, b.slots, kv.k[li], kv.v[li])
+        if self.kv8:
+            fn = ck.qk_norm_rope_kv_append_kv8_splitk if splits else ck.qk_norm_rope_kv_append_kv8
+            fn(desc, *head, *tail, kv.k_scale[li], kv.v_scale[li], self.q[:T], gate)
+        else:
+            fn = ck.qk_norm_rope_kv_append_splitk if splits else ck.qk_norm_rope_kv_append
+            fn(desc, *head, *tail, self.q[:T], gate)
+
+    def _attend(self, desc, li: int, b: VerifyBatch, T: int, workspace=None) -> None:
+        kv, gate = self.kv, self.gate[:T] if self.shape.gated else None
+        if self.kv8:
+            ck.paged_attention_verify_kv8(desc, self.q[:T], kv.k[li], kv.v[li], kv.k_scale[li], kv.v_scale[li],
+                                          b.block_table, b.cu_q, b.context_lens, gate, self.attn[:T],
+                                          window=self.window, sinks=self.sinks, workspace=workspace)
+        else:
+            ck.paged_attention_verify(desc, self.q[:T], kv.k[li], kv.v[li], b.block_table, b.cu_q, b.context_lens, gate,
+                                      self.attn[:T])
+
     def forward(self, b: VerifyBatch) -> torch.Tensor:
         """Post-final-norm hidden states [T, H] (Qwen3Model.forward, return_last_hidden)."""
         s = self.shape
@@ -431,6 +511,7 @@ class Qwen3Verifier:
         res, h = self.residual[:T], self.h[:T]
         ck.embedding_bf16(b.ids, self.w.embed, out=res)
         part = self.part if self.defer_splitk else None
+        workspace = self._kv8_workspace(desc) if self.kv8 else None
 
         def linear(lin, x, out) -> int:  # split count of partials left in part, else 0 (out written)
             if part is None:
@@ -451,16 +532,9 @@ class Qwen3Verifier:
             sp = linear(L["qkv"], h, self.qkv[:T])
             if e is not None:
                 e.record()
-            gate = self.gate[:T] if s.gated else None
-            if sp:
-                ck.qk_norm_rope_kv_append_splitk(desc, part, sp, L["q_norm"], L["k_norm"], self.cos, self.sin,
-                                                 b.positions, b.slots, self.kv.k[li], self.kv.v[li], self.q[:T], gate)
-            else:
-                ck.qk_norm_rope_kv_append(desc, self.qkv[:T], L["q_norm"], L["k_norm"], self.cos, self.sin,
-                                          b.positions, b.slots, self.kv.k[li], self.kv.v[li], self.q[:T], gate)
+            self._append(desc, li, L, b, part, sp)
             e = self._ev("attention")
-            ck.paged_attention_verify(adesc, self.q[:T], self.kv.k[li], self.kv.v[li], ab.block_table, ab.cu_q,
-                                      ab.context_lens, self.gate[:T] if s.gated else None, self.attn[:T])
+            self._attend(adesc, li, ab, T, workspace)
             if e is not None:
                 e.record()
             e = self._ev("linear_o")
@@ -488,12 +562,11 @@ class Qwen3Verifier:
         s = self.shape
         T = b.total_q
         desc = self._desc(b)
-        gate = self.gate[:T] if s.gated else None
+        workspace = self._kv8_workspace(desc) if self.kv8 else None
 
         def body():
             for li in range(s.layers):
-                ck.paged_attention_verify(desc, self.q[:T], self.kv.k[li], self.kv.v[li], b.block_table, b.cu_q,
-                                          b.context_lens, gate, self.attn[:T])
+                self._attend(desc, li, b, T, workspace)
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -679,13 +752,16 @@ class VerifyGraph:
         self.graph.replay()
 
 
-def attention_bytes(shape: Qwen3Shape, context_lens: list[int], q_lens: list[int]) -> int:
+def attention_bytes(shape: Qwen3Shape, context_lens: list[int], q_lens: list[int], kv_bytes: int = 2) -> int:
     """Algorithmic HBM bytes of one layer's paged attention: every key/value of each
-    sequence once, the queries and outputs, and the appended K/V rows."""
-    kv = sum(context_lens) * shape.n_kv_heads * shape.head_dim * 2 * 2
+    sequence once (kv_bytes per element; 1: the 8-bit cache, whose page scales count too),
+    the queries and outputs, and the appended K/V rows."""
+    kv = sum(context_lens) * shape.n_kv_heads * shape.head_dim * kv_bytes * 2
+    if kv_bytes == 1:
+        kv += sum(-(-c // shape.block_size) for c in context_lens) * shape.n_kv_heads * 4 * 2
     rows = sum(q_lens)
     qo = rows * shape.n_heads * shape.head_dim * 2 * 2
-    app = rows * shape.n_kv_heads * shape.head_dim * 2 * 2
+    app = rows * shape.n_kv_heads * shape.head_dim * kv_bytes * 2
     return kv + qo + app
 
 
@@ -776,7 +852,7 @@ class Qwen3VerifierF32(Qwen3Verifier):
     the same structure as Qwen3Verifier with the fp32 kernels; fp32 logits."""
 
     def __init__(self, weights: Qwen3WeightsF32, kv: PagedKVCache, max_rows: int, max_pos: int, device):
-        if kv.dtype != torch.float32:
+        if kv.dtype != torch.float32:  # the 8-bit cache neither
             raise ValueError("the fp32 verifier needs an fp32 KV cache")
         super().__init__(weights, kv, max_rows, max_pos, device)
         s = self.shape
