@@ -89,6 +89,38 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
+// two floats at once
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
 // Probabilities are held as 2^9 exp(s - m) in f16 for a reference m at most kLag below the running
 // maximum (in base 2): at most 2^15, with 11 bits down to 2^-23 of exp(m) and steps of 2^-33 below,
@@ -520,12 +552,27 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                             }
                 }
                 // ---- scores in base 2, masks, online softmax ----
+                // A page's K scale is a factor of its raw products, applied with the reference in one
+                // fma; its V scale is an addend there (p' = p * vs / vref), taken out of the sum again.
+                float f[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) f[i][0] = rowf[0] * kf[i], f[i][1] = rowf[1] * kf[i];
                 int key0[2] = {0, 0};
+                auto scale_scores = [&]() {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) s[i][t][j] *= f[i][j >> 1];
+                        f[i][0] = f[i][1] = 1.f;
+                    }
+                };
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const bool ok_page = (valid >> i) & 1u;
-                        if (!ok_page) kf[i] = vf[i] = 0.f;
+                        if (!ok_page) vf[i] = 0.f;
                         key0[i] = page_of(g, vp + i) * 16;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
@@ -535,39 +582,36 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                                 const bool see = vp + i < g.nv && key <= qp &&
                                                  (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
                                 // a page with no valid id is one of zeros
-                                s[i][t][j] = see ? (ok_page ? s[i][t][j] * (rowf[j >> 1] * kf[i]) : 0.f) : -INFINITY;
+                                s[i][t][j] = see ? (ok_page ? s[i][t][j] * f[i][j >> 1] : 0.f) : -INFINITY;
                             }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float f[2] = {rowf[0] * kf[i], rowf[1] * kf[i]};
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) s[i][t][j] *= f[j >> 1];
+                        f[i][0] = f[i][1] = 1.f;
                     }
                 }
                 float mx[2];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    mx[hh] = fmaxf(fmaxf(fmaxf(s[0][0][2 * hh], s[0][0][2 * hh + 1]), fmaxf(s[0][1][2 * hh], s[0][1][2 * hh + 1])),
-                                   fmaxf(fmaxf(s[1][0][2 * hh], s[1][0][2 * hh + 1]), fmaxf(s[1][1][2 * hh], s[1][1][2 * hh + 1])));
+                    const int e = 2 * hh;
+                    mx[hh] = fmaxf(fmaxf(max3(s[0][0][e], s[0][0][e + 1], s[0][1][e]), s[0][1][e + 1]) * f[0][hh],
+                                   fmaxf(max3(s[1][0][e], s[1][0][e + 1], s[1][1][e]), s[1][1][e + 1]) * f[1][hh]);
                     mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
                     mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
                 }
                 const float vtop = fmaxf(vref, fmaxf(vf[0], vf[1]));
-                if (__any_sync(0xffffffffu, mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || vtop > vref)) {
+                // (the fma adds -m to an unrounded product, off by half a unit of m: scores past 2^16
+                // are rounded first, like m)
+                const bool huge = fabsf(mx[0]) > 65536.f || fabsf(mx[1]) > 65536.f;
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || vtop > vref || huge)) {
+                    if (!masked && __any_sync(0xffffffffu, huge)) scale_scores();
                     const float inv = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
                     const float vfac = vref * inv;
                     vref = vtop, inv_vref = inv;
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         const float mn = fmaxf(m[hh], mx[hh]);
-                        const float f = mn == m[hh] ? 1.f : ex2(m[hh] - mn);  // first keys: ex2(-inf) = 0
+                        const float fm = mn == m[hh] ? 1.f : ex2(m[hh] - mn);  // first keys: ex2(-inf) = 0
                         m[hh] = mn;
-                        l[hh] *= f;
-                        const float fo = f * vfac;
+                        l[hh] *= fm;
+                        const float fo = fm * vfac;
 #pragma unroll
                         for (int n = 0; n < 16; ++n) o[n][2 * hh] *= fo, o[n][2 * hh + 1] *= fo;
                     }
@@ -577,16 +621,19 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                 uint32_t pa[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float r = vf[i] * inv_vref;
+                    // a page whose scale is 2^-60 of the largest or less counts for nothing in O
+                    const float lr = fmaxf(lg2(vf[i] * inv_vref), -60.f), back = ex2(-lr);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const uint64_t ff = f2_pack(f[i][hh], f[i][hh]), cc = f2_pack(base[hh] + lr, base[hh] + lr);
+                        float2 x[2];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            s[i][t][j] = ex2(s[i][t][j] + base[j >> 1]);
-                            l[j >> 1] += s[i][t][j];
+                        for (int t = 0; t < 2; ++t) {
+                            x[t] = f2_unpack(f2_fma(f2_pack(s[i][t][2 * hh], s[i][t][2 * hh + 1]), ff, cc));
+                            x[t].x = ex2(x[t].x), x[t].y = ex2(x[t].y);
+                            pa[i][2 * t + hh] = pack_f16(x[t].x, x[t].y);
                         }
-                        pa[i][2 * t] = pack_f16(s[i][t][0] * r, s[i][t][1] * r);
-                        pa[i][2 * t + 1] = pack_f16(s[i][t][2] * r, s[i][t][3] * r);
+                        l[hh] = fmaf((x[0].x + x[0].y) + (x[1].x + x[1].y), back, l[hh]);
                     }
                 }
                 // ---- O += P V8 ----
@@ -929,32 +976,6 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// two floats at once
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
 // the largest of 16 floats
 __device__ __forceinline__ float max16(const uint32_t *s) {
     float a = max3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
@@ -965,12 +986,6 @@ __device__ __forceinline__ float max16(const uint32_t *s) {
     b = max3(b, __uint_as_float(s[14]), __uint_as_float(s[15]));
     return fmaxf(max3(a, b, c), d);
 }
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 struct __align__(8) ChunkBars {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done;
 };
