@@ -247,6 +247,26 @@ def lib():
     return _load_lib()
 
 
+_args = None
+
+
+def args():
+    """The extension module that checks tensors and makes the 8-bit KV cache calls (csrc/args.cpp),
+    bound to the loaded library.  Raises when it has not been built."""
+    global _args
+    if _args is None:
+        try:
+            from . import _args as module
+        except ImportError as e:
+            raise RuntimeError("pilm_b200/_args.so could not be loaded: build it with `python -m pilm_b200.build`") from e
+        L = _load_lib()
+        module.bind(*(ctypes.cast(getattr(L, n), _vp).value for n in
+                      ("ekernel_qk_norm_rope_kv_append_kv8", "ekernel_qk_norm_rope_kv_append_kv8_splitk",
+                       "ekernel_paged_attention_verify_kv8")))
+        _args = module
+    return _args
+
+
 def last_error() -> str:
     e = _load_lib().ecpu_last_error()
     return e.decode() if e else ""

@@ -2,6 +2,9 @@
 
     python -m pilm_b200.build            # or: import pilm_b200.build; build()
 
+and _args.so, the Python entry of the 8-bit KV cache calls (csrc/args.cpp), with g++ against
+torch's headers.
+
 The library is written next to this file so that it ships with the package and
 with snapshots of the repository; it is rebuilt only when a source is newer.
 """
@@ -16,6 +19,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libpilm_cuda.so"
+ARGS = HERE / "_args.so"
 INCLUDE = HERE.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["runtime.cu", "linear.cu", "linear_tc.cu", "norm.cu", "attention.cu", "accept.cu", "mtp.cu", "f32.cu",
@@ -37,7 +41,29 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > t for p in deps if p.exists())
 
 
+def build_args(force: bool = False) -> Path:
+    """_args.so: a Python extension module on torch's C++ API."""
+    src = CSRC / "args.cpp"
+    deps = [src] + list(INCLUDE.glob("*.h"))
+    if not force and ARGS.exists() and all(p.stat().st_mtime <= ARGS.stat().st_mtime for p in deps):
+        return ARGS
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    tmp = ARGS.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), str(src),
+           "-L", str(root / "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", str(tmp)]
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, ARGS)
+    return ARGS
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_args(force)
     if not force and not _stale():
         return LIB
     objdir = HERE / "_build"

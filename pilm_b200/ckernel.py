@@ -382,56 +382,21 @@ def paged_attention_verify(desc, q, k_cache, v_cache, block_table, cu_q, context
 
 # ---- 8-bit KV cache: e4m3 codes, one scale per page and KV head ----------------------------
 
-# These calls are a few microseconds each on small batches, and a serving loop makes one of each per
-# layer: the checks below are written for few Python operations per tensor.
-
-def _kv8_bad(name, t, dtype, numel, dev) -> None:
+def _kv8_call(k_cache, what: str, fn, *args) -> None:
+    """fn(device, *args) on the device's current stream, with the tensors' device current; fn checks
+    the tensors (ValueError) and returns the C call's code."""
+    dev = k_cache.get_device()
     if dev < 0:
-        raise ValueError(f"{name}: the 8-bit cache calls take CUDA tensors")
-    raise ValueError(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements on cuda:{dev}, got "
-                     f"{t.dtype} {tuple(t.shape)} on {t.device}" + ("" if t.is_contiguous() else " (not contiguous)"))
-
-
-def _kv8_ptr(name: str, t: torch.Tensor, dtype: torch.dtype, numel: int, dev: int) -> int:
-    """The address of a tensor that the kernels reach by raw pointer: contiguous, of the dtype, on
-    the call's device, with at least numel elements."""
-    if t.dtype is not dtype or t.numel() < numel or t.get_device() != dev or dev < 0 or not t.is_contiguous():
-        _kv8_bad(name, t, dtype, numel, dev)
-    return t.data_ptr()
-
-
-def _kv8_cache(desc, dev: int, k_cache, v_cache, k_scale, v_scale):
-    n = desc.num_blocks * desc.n_kv_heads
-    codes = n * desc.block_size * desc.head_dim
-    u8, f32 = torch.uint8, torch.float32
-    return (_kv8_ptr("k_cache", k_cache, u8, codes, dev), _kv8_ptr("v_cache", v_cache, u8, codes, dev),
-            _kv8_ptr("k_scale", k_scale, f32, n, dev), _kv8_ptr("v_scale", v_scale, f32, n, dev))
-
-
-def _kv8_call(dev: int, what: str, fn, *args) -> None:
-    """The call on the device's current stream, with the tensors' device current."""
-    if torch._C._cuda_getDevice() != dev:
+        raise ValueError("the 8-bit cache calls take CUDA tensors")
+    if torch._C._cuda_getDevice() == dev:
+        abi.set_stream(torch._C._cuda_getCurrentRawStream(dev))
+        rc = fn(dev, *args)
+    else:
         with torch.cuda.device(dev):
             abi.set_stream(torch.cuda.current_stream().cuda_stream)
-            rc = fn(*args)
-    else:
-        abi.set_stream(torch._C._cuda_getCurrentRawStream(dev))
-        rc = fn(*args)
+            rc = fn(dev, *args)
     if rc:
         _check(rc, what)
-
-
-def _append_kv8_args(desc, dev: int, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache,
-                     k_scale, v_scale, q_out, gate_out):
-    hd, t = desc.head_dim, desc.total_q
-    rows, nf = t * desc.n_heads * hd, desc.rope_rows * (desc.rot_dim // 2)
-    bf, f32, i32 = torch.bfloat16, torch.float32, torch.int32
-    cache = _kv8_cache(desc, dev, k_cache, v_cache, k_scale, v_scale)
-    return (_kv8_ptr("q_norm_w", q_norm_w, bf, hd, dev), _kv8_ptr("k_norm_w", k_norm_w, bf, hd, dev),
-            _kv8_ptr("rope_cos", rope_cos, f32, nf, dev), _kv8_ptr("rope_sin", rope_sin, f32, nf, dev),
-            _kv8_ptr("positions", positions, i32, t, dev), _kv8_ptr("slot_mapping", slot_mapping, i32, t, dev), *cache,
-            _kv8_ptr("q_out", q_out, bf, rows, dev),
-            _kv8_ptr("gate_out", gate_out, bf, rows, dev) if desc.output_gate and gate_out is not None else None)
 
 
 def qk_norm_rope_kv_append_kv8(desc, qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache,
@@ -440,23 +405,18 @@ def qk_norm_rope_kv_append_kv8(desc, qkv, q_norm_w, k_norm_w, rope_cos, rope_sin
     pages of an 8-bit cache (uint8 e4m3 codes [num_blocks, 16, n_kv, 128], fp32 scales
     [num_blocks, n_kv]; see include/pilm_cuda.h for the scale's rule).  Written: q_out, gate_out
     when the descriptor is gated, the caches and scales."""
-    dev = k_cache.get_device()
-    src = _kv8_ptr("qkv", qkv, torch.bfloat16, desc.total_q * desc.qkv_stride, dev)
-    args = _append_kv8_args(desc, dev, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache,
-                            k_scale, v_scale, q_out, gate_out)
-    _kv8_call(dev, "ekernel_qk_norm_rope_kv_append_kv8", abi.lib().ekernel_qk_norm_rope_kv_append_kv8, desc, src, *args)
+    _kv8_call(k_cache, "ekernel_qk_norm_rope_kv_append_kv8", abi.args().append, desc, qkv, 0, q_norm_w, k_norm_w, rope_cos,
+              rope_sin, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out, gate_out)
 
 
 def qk_norm_rope_kv_append_kv8_splitk(desc, partials, splits, q_norm_w, k_norm_w, rope_cos, rope_sin, positions,
                                       slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out, gate_out=None) -> None:
     """qk_norm_rope_kv_append_kv8 with the projection given as a deferred W4 linear's split-K
     partial sums ([splits, total_q, qkv_stride] fp32)."""
-    dev = k_cache.get_device()
-    src = _kv8_ptr("partials", partials, torch.float32, splits * desc.total_q * desc.qkv_stride, dev)
-    args = _append_kv8_args(desc, dev, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache,
-                            k_scale, v_scale, q_out, gate_out)
-    _kv8_call(dev, "ekernel_qk_norm_rope_kv_append_kv8_splitk", abi.lib().ekernel_qk_norm_rope_kv_append_kv8_splitk, desc,
-              src, int(splits), *args)
+    if splits < 1:
+        raise ValueError(f"splits must be positive, got {splits}")
+    _kv8_call(k_cache, "ekernel_qk_norm_rope_kv_append_kv8_splitk", abi.args().append, desc, partials, splits, q_norm_w,
+              k_norm_w, rope_cos, rope_sin, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out, gate_out)
 
 
 def _window(window: int, sinks: int) -> None:
@@ -476,19 +436,11 @@ def paged_attention_verify_kv8(desc, q, k_cache, v_cache, k_scale, v_scale, bloc
     window > 0 a row at position p sees the keys in (p - window, p] and the first `sinks`.
     workspace: a uint8 tensor of paged_attention_kv8_workspace_bytes; allocated here when None.
     Calls that may run at the same time need workspaces of their own."""
-    _window(window, sinks)
-    dev, rows = k_cache.get_device(), desc.total_q * desc.n_heads * desc.head_dim
-    bf, i32, seqs = torch.bfloat16, torch.int32, desc.num_seqs
-    cache = _kv8_cache(desc, dev, k_cache, v_cache, k_scale, v_scale)
     if workspace is None:
         workspace = torch.empty(paged_attention_kv8_workspace_bytes(desc, window, sinks), dtype=torch.uint8,
                                 device=k_cache.device)
-    _kv8_call(dev, "ekernel_paged_attention_verify_kv8", abi.lib().ekernel_paged_attention_verify_kv8, desc,
-              _kv8_ptr("q", q, bf, rows, dev), *cache,
-              _kv8_ptr("block_table", block_table, i32, seqs * desc.max_blocks_per_seq, dev),
-              _kv8_ptr("cu_q", cu_q, i32, seqs + 1, dev), _kv8_ptr("context_lens", context_lens, i32, seqs, dev),
-              _kv8_ptr("gate", gate, bf, rows, dev) if desc.output_gate and gate is not None else None, window, sinks,
-              _kv8_ptr("workspace", workspace, torch.uint8, 0, dev), workspace.numel(), _kv8_ptr("out", out, bf, rows, dev))
+    _kv8_call(k_cache, "ekernel_paged_attention_verify_kv8", abi.args().attention, desc, q, k_cache, v_cache, k_scale,
+              v_scale, block_table, cu_q, context_lens, gate, out, window, sinks, workspace)
 
 
 # ---- fp32-activation path (the W8A32 configuration) --------------------------------------

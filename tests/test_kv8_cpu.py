@@ -104,6 +104,28 @@ def test_wrappers_refuse_cpu_tensors():
         ck.qk_norm_rope_kv_append_kv8(desc(), t, t, t, s, s, t, t, t, t, s, s, t)
 
 
+def test_argument_module_refuses_what_is_no_call():
+    m, t = abi.args(), torch.zeros(1)
+    with pytest.raises(TypeError):
+        m.append(0, desc())
+    with pytest.raises(TypeError):
+        m.attention(*range(14))
+    with pytest.raises(ValueError, match="PagedAttnDesc"):
+        m.append(0, b"short", t, 0, *[t] * 12)
+    with pytest.raises(TypeError):
+        m.append(0, object(), t, 0, *[t] * 12)
+    with pytest.raises(ValueError, match="qkv must be a tensor"):
+        m.append(0, desc(), 5, 0, *[t] * 12)
+    with pytest.raises(ValueError, match="qkv must be a contiguous"):
+        m.append(0, desc(), t, 0, *[t] * 12)
+    with pytest.raises(ValueError, match="negative"):
+        m.attention(0, desc(), *[t] * 10, -1, 0, t)
+    with pytest.raises(ValueError, match="CUDA"):  # a tensor without storage
+        m.append(0, desc(), torch.zeros(1024, dtype=torch.bfloat16, device="meta"), 0, *[t] * 12)
+    with pytest.raises(ValueError):
+        m.bind(1, 2, 0)
+
+
 # ---- the restatement -------------------------------------------------------------------------
 
 def test_restated_scales_and_steps():
