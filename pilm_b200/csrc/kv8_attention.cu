@@ -87,29 +87,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-
-// two floats at once
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 f2_unpack(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -1394,25 +1371,43 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     }
 }
 
-// Adds the splits of the chunk kernel.  A warp per (row, query head), lane l: dims 4l .. 4l + 3.
+// Adds the splits of the chunk kernel.  WPI warps per (row, query head), each over every WPI-th
+// split, lane l: dims 4l .. 4l + 3; the first one adds their sums.
+template <int WPI>
 __global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int num_seqs) {
+    __shared__ float4 s_o[8][32];
+    __shared__ float2 s_ml[8];
     pdl_trigger();
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % WPI;
+    const long long item = (long long)blockIdx.x * (8 / WPI) + warp / WPI;
     // rows of the batch only: those behind the last sequence are not written
-    if (item >= (long long)p.geo.cu_q[num_seqs] * p.nh || item < (long long)p.geo.cu_q[0] * p.nh) return;
+    const bool in = item < (long long)p.geo.cu_q[num_seqs] * p.nh && item >= (long long)p.geo.cu_q[0] * p.nh;
     float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-        const float *rec = p.part + ((size_t)s * p.total_q * p.nh + item) * kRec;
-        const float m = rec[kHD], l = rec[kHD + 1];
-        const float4 o = *reinterpret_cast<const float4 *>(rec + 4 * lane);
+    auto add = [&](float m, float l, const float4 &o) {
         const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.f : mn;
         const float f = ex2(M - mb), w = l * ex2(m - mb);
         M = mn, L = L * f + w;
         O[0] = O[0] * f + w * o.x, O[1] = O[1] * f + w * o.y, O[2] = O[2] * f + w * o.z, O[3] = O[3] * f + w * o.w;
+    };
+    if (in) {
+#pragma unroll 4
+        for (int s = part; s < p.splits; s += WPI) {
+            const float *rec = p.part + ((size_t)s * p.total_q * p.nh + item) * kRec;
+            add(rec[kHD], rec[kHD + 1], *reinterpret_cast<const float4 *>(rec + 4 * lane));
+        }
     }
+    if (WPI > 1) {
+        // a partial sum as a record: O / L with weight L
+        const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
+        s_o[warp][lane] = make_float4(O[0] * f, O[1] * f, O[2] * f, O[3] * f);
+        if (lane == 0) s_ml[warp] = make_float2(M, L);
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int i = 1; i < WPI; ++i) add(s_ml[warp + i].x, s_ml[warp + i].y, s_o[warp + i][lane]);
+    }
+    if (!in) return;
     const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
     finish4(p.out, p.gate, (size_t)item * kHD + 4 * lane, O, f);
 }
@@ -1485,9 +1480,12 @@ struct ChunkPlan {
     size_t part_bytes;
 };
 
-// Calls of many rows per KV head run on the chunk kernel.  Its 128-row tiles cost the same however
-// few of their rows are used, and the token kernel's 16-row tiles each convert the cache anew.
-constexpr long long kChunkRows = 96;
+// Calls of more than 32 rows per KV head run on the chunk kernel.  Its 128-row tiles cost the same
+// however few of their rows are used; the token kernel converts the cache anew for every 16-row tile
+// and reads it anew for every eight.  Measured (us, token against chunk): 32 sequences over 8K keys,
+// 8 KV heads, 32 rows 167 against 239, 40 rows 309 against 240; 24 sequences over 2.5K keys, 2 KV
+// heads, 40 rows 31 against 24; one sequence of 40 rows over 8K keys 14.6 against 15.9.
+constexpr long long kChunkRows = 33;
 
 bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks, ChunkPlan &c) {
     const int gsz = (int)(d->n_heads / d->n_kv_heads);
@@ -1501,9 +1499,10 @@ bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks
         if (seen < keys) keys = seen;
     }
     const long long blocks = (keys + kChKeys - 1) / kChKeys;
-    // fewer CTAs than SMs: split the keys, at least four blocks each
-    long long s = (num_sms() + ctas - 1) / ctas;
-    if (s > blocks / 4) s = blocks / 4;
+    // fewer CTAs than SMs: split the keys as far as one wave of CTAs goes (1000 rows over 8K keys, 2 KV
+    // heads: 96 us; one split more, of two waves, 126), at least three blocks each
+    long long s = num_sms() / ctas;
+    if (s > blocks / 3) s = blocks / 3;
     c.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
     c.part_bytes = c.splits > 1 ? (size_t)c.splits * d->total_q * d->n_heads * kRec * sizeof(float) : 0;
     return ctas * c.splits <= 0x7fffffffLL;
@@ -1602,7 +1601,10 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         if (rc == ECPU_OK) rc = check_error(what);
         if (rc != ECPU_OK || c.splits == 1) return rc;
         const size_t items = desc->total_q * desc->n_heads;
-        launch_pdl(kv8_attn_join, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, p, (int)desc->num_seqs);
+        if (c.splits > 4 && items <= (size_t)num_sms() * 8)  // few rows of many splits: 8 warps share a row's
+            launch_pdl(kv8_attn_join<8>, dim3((unsigned)items), dim3(256), 0, p, (int)desc->num_seqs);
+        else
+            launch_pdl(kv8_attn_join<1>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, p, (int)desc->num_seqs);
         return check_launch(what);
     }
     const TokPlan t = plan_tokens(desc, window, sinks);
@@ -1648,12 +1650,16 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         if (t.G == 1 || t.whole) continue;  // every group whole
         // a row of the batch is the longest a sequence can have
         const int max_q = (int)(desc->max_q_len < 1 ? 1 : (desc->max_q_len < desc->total_q ? desc->max_q_len : desc->total_q));
-        // few groups over many CTAs: all of a block's warps on one row and head's partials
-        const bool wide = t.G > 16 * seqs * t.rgs;
-        const int per = wide ? 1 : 8;
+        // A group's partials lie in span CTAs at most.  As many warps share a row and head as load them
+        // in one round (8 sequences of 5 rows over 4K keys: 38.0 us with 16 warps, 24.6 with 4); 16
+        // with 10 loads each where one wave of blocks holds them all (8 rows over 8K: 20.2 against 21.1).
+        const int span = t.G / (seqs * t.rgs) + 2;
+        const bool wide = span > 8 && (long long)max_q * p.nh * seqs <= num_sms();
+        int wpi = wide ? 16 : 1;
+        while (!wide && wpi < 8 && 8 * wpi < span) wpi *= 2;
+        const int per = wide ? 1 : 8 / wpi;
         launch_pdl(wide ? kv8_attn_merge<16, 10> : kv8_attn_merge<8, 8>,
-                   dim3((unsigned)((p.nh + per - 1) / per * max_q), (unsigned)seqs), dim3(wide ? 512 : 256), 0, p,
-                   wide ? 16 : 1);
+                   dim3((unsigned)((p.nh + per - 1) / per * max_q), (unsigned)seqs), dim3(wide ? 512 : 256), 0, p, wpi);
         rc = check_launch(what);
         if (rc != ECPU_OK) return rc;
     }

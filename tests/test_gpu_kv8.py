@@ -297,6 +297,13 @@ def test_attention_many_ragged_sequences():
     attn_case(q, [n + rnd.randint(0, 900) for n in q], 32, 8, seed=8, gated=True)
 
 
+@pytest.mark.parametrize("seqs,rows,nh,nkv", [(2, 4, 32, 8), (3, 5, 16, 8), (8, 1, 16, 2), (8, 3, 16, 2), (12, 4, 32, 8),
+                                              (20, 1, 8, 1), (1, 8, 32, 8), (1, 40, 8, 8), (2, 20, 8, 4), (30, 9, 32, 8)])
+def test_attention_sequence_counts(seqs, rows, nh, nkv):
+    """From one sequence over all SMs to a few SMs for each: the shares of a row meet in every way."""
+    attn_case([rows - (i % 2 and rows > 1) for i in range(seqs)], [2900 - 97 * i for i in range(seqs)], nh, nkv, seed=seqs)
+
+
 def test_attention_more_sequences_than_one_launch_indexes():
     attn_case([1] * 5000, [1 + (i * 7) % 40 for i in range(5000)], 2, 2, seed=9)
 
