@@ -953,6 +953,8 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// the lowest n of 16 bits, none for n <= 0, all for n >= 16
+__device__ __forceinline__ uint32_t low16(int n) { return (1u << min(max(n, 0), 16)) - 1u; }
 // the largest of 16 floats
 __device__ __forceinline__ float max16(const uint32_t *s) {
     float a = max3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
@@ -1011,12 +1013,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     const int rho0 = rg * kChRows, rho1 = min(q_len * gsz, rho0 + kChRows);
     const int tiles = rho1 - rho0 > kChTile ? 2 : (rho1 > rho0 ? 1 : 0);
     // blocks of the group: n_sink from the first key on, then those from lo on
-    int n_sink = 0, lo = 0, nb = 0;
+    int n_sink = 0, lo = 0, nb = 0, first = 0;  // first: the page of the first key within a window
     if (tiles > 0) {
         const int pmin = p0 + rho0 / gsz, pmax = p0 + (rho1 - 1) / gsz;
         if (pmax >= 0) {
             if (p.geo.window > 0) {
-                lo = max(0, pmin - p.geo.window + 1) / kChKeys;
+                first = max(0, pmin - p.geo.window + 1) / kKv8Page * kKv8Page;
+                lo = first / kChKeys;
                 n_sink = min((p.geo.sinks + kChKeys - 1) / kChKeys, lo);
             }
             nb = n_sink + pmax / kChKeys + 1 - lo;
@@ -1105,7 +1108,9 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             int blk = -1;
             if (j < j1 && lane < 8) {
                 const int pg = key_of(j) / kKv8Page + lane;
-                if (pg < p.max_blocks && pg * kKv8Page < ctx) blk = bt[pg];
+                // past the context, or wholly outside the rows' windows (its id may be another's by now)
+                if (pg < p.max_blocks && pg * kKv8Page < ctx && (pg * kKv8Page >= first || pg * kKv8Page < p.geo.sinks))
+                    blk = bt[pg];
                 if (blk < 0 || blk >= p.num_blocks) blk = -1;
             }
             return blk;
@@ -1234,37 +1239,52 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                     for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i], vtop = fmaxf(vtop, c2[i]);
                 }
                 const int key0 = key_of(j);
-                bool plain = key0 + kChKeys - 1 <= pmin &&
-                             (p.geo.window == 0 || key0 > pmax - p.geo.window || key0 + kChKeys - 1 < p.geo.sinks);
-                float mx = -INFINITY;
-                if (plain) {  // the maximum, page by page on the raw products
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t s[64];
-                        tc_ld32(s_at + 64 * c, s);
-                        tc_ld32(s_at + 64 * c + 32, s + 32);
+                auto seen_whole = [&](int k0, int keys) {  // by all rows of the warp
+                    return k0 + keys - 1 <= pmin &&
+                           (p.geo.window == 0 || k0 > pmax - p.geo.window || k0 + keys - 1 < p.geo.sinks);
+                };
+                const bool plain = seen_whole(key0, kChKeys);
+                if (!plain) {
+                    // in pages that some row does not see whole, which at 128 keys a block are few, the
+                    // others' scores become -inf, which must not meet a factor of 0 (with the least
+                    // normal number in its place a product is still nothing beside the exponents)
+#pragma unroll 1
+                    for (int i = 0; i < 8; ++i) {
+                        const int k0 = key0 + 16 * i;
+                        if (seen_whole(k0, 16)) continue;
+                        uint32_t s[16], see = low16(qp + 1 - k0);
+                        if (p.geo.window) see &= ~low16(qp - p.geo.window + 1 - k0) | low16(p.geo.sinks - k0);
+                        tc_ld16(s_at + 16 * i, s);
                         tc_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, max16(s + 16 * i) * f[4 * c + i]);
+                        for (int k = 0; k < 16; ++k)
+                            if (!((see >> k) & 1u)) s[k] = 0xff800000u;
+                        tc_st16(s_at + 16 * i, s);
                     }
-                    // The fma below adds -m to an unrounded product: off by half a unit of m, which
-                    // must stay far below 1.  Scores past 2^16 are rounded first, like m.
-                    plain = !__any_sync(0xffffffffu, fabsf(mx) > 65536.f);
+                    tc_st_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = fmaxf(f[i], 1.17549435e-38f);
                 }
-                if (!plain) {  // scaled scores (a factor of 0 must not meet an infinity), masked ones -inf
-                    mx = -INFINITY;
+                float mx = -INFINITY;  // page by page on the raw products
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t s[64];
+                    tc_ld32(s_at + 64 * c, s);
+                    tc_ld32(s_at + 64 * c + 32, s + 32);
+                    tc_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, max16(s + 16 * i) * f[4 * c + i]);
+                }
+                // The fma below adds -m to an unrounded product: off by half a unit of m, which
+                // must stay far below 1.  Scores past 2^16 are rounded first, like m.
+                if (__any_sync(0xffffffffu, fabsf(mx) > 65536.f && mx > -INFINITY)) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t s[32];
                         tc_ld32(s_at + 32 * c, s);
                         tc_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int key = key0 + 32 * c + i;
-                            const bool see = key <= qp && (p.geo.window == 0 || key > qp - p.geo.window || key < p.geo.sinks);
-                            s[i] = __float_as_uint(see ? __uint_as_float(s[i]) * f[2 * c + (i >> 4)] : -INFINITY);
-                        }
-                        mx = max3(mx, max16(s), max16(s + 16));
+                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f[2 * c + (i >> 4)]);
                         tc_st32(s_at + 32 * c, s);
                     }
 #pragma unroll
