@@ -19,7 +19,7 @@ static __device__ int g_kv8_error;
 namespace {
 
 constexpr int kHD = kKv8HD;
-constexpr uint32_t kWaitLimit = 1u << 22;  // polls before a wait gives up
+constexpr uint32_t kWaitLimit = 1u << 20;  // polls, of about two microseconds each, before a wait gives up
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t count) {
@@ -42,11 +42,11 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait; false once the limit is reached or another warp gave up.
+// Bounded wait; false once the limit is reached or another warp gave up (unless abort_flag is null).
 __device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag) {
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         if (mbar_try_wait(b, parity)) return true;
-        if ((i & 255) == 255 && *abort_flag) return false;
+        if (abort_flag && (i & 255) == 255 && *abort_flag) return false;
     }
     return false;
 }
@@ -382,9 +382,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         }
         // every copy issued lands before the CTA may exit
         for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
-            for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&full_bar[j % p.stages], (uint32_t)(j / p.stages) & 1u);
-                 ++i) {
-            }
+            mbar_wait(&full_bar[j % p.stages], (uint32_t)(j / p.stages) & 1u, nullptr);
         return;
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -1093,8 +1091,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             // everything issued has completed (also when a wait gave up)
             if (lane == 0) tc_commit(&bar.o_done);
             __syncwarp();
-            bool done = false;
-            for (uint32_t i = 0; i < kWaitLimit && !done; ++i) done = mbar_try_wait(&bar.o_done, 0);
+            mbar_wait(&bar.o_done, 0, nullptr);
             if (!ok && lane == 0) atomicExch(&g_kv8_error, 1);
             __syncwarp();
         }
