@@ -343,6 +343,71 @@ def test_invalid_block_ids_read_as_zeros(rows):
     attn_case([rows, rows], [rows + 300, rows + 65], 8, 2, seed=rows, edit=edit)
 
 
+@pytest.mark.parametrize("rows", [2, 12, 150])
+def test_pages_outside_the_windows_are_not_looked_at(rows):
+    """A serving loop frees pages that have left every row's window: their table entries may be
+    anything, another owner's page or one of NaN codes and scales, and no bit changes."""
+    d, nh, nkv, window, sinks, ctx = dev(), 16, 2, 300, 20, 2500
+    b = ref.batch([rows, 1], [ctx, ctx - 900], rows)
+    g = torch.Generator(device=d).manual_seed(rows)
+    q = torch.randn((b.total, nh * HD), generator=g, device=d).to(torch.bfloat16)
+    kc, vc, ks, vs = ref.random_cache(b.blocks + 1, nkv, 3, d)
+    for t, bad in ((kc, 0x7F), (vc, 0xFF), (ks, math.nan), (vs, math.nan)):
+        t[b.blocks] = bad
+    desc = make_desc(b, nh, nkv)
+    desc.num_blocks = b.blocks + 1
+    table = table_of(b)
+    outs = []
+    for freed in (False, True):
+        if freed:
+            for i, (n, c) in enumerate(zip(b.q_lens, b.ctxs)):
+                for pg in range(-(-sinks // PAGE), (c - n - window + 1) // PAGE):
+                    table[i, pg] = (b.blocks, -1, 0, 2 ** 31 - 1)[pg % 4]
+        out = torch.empty((b.total, nh * HD), dtype=torch.bfloat16, device=d)
+        ck.paged_attention_verify_kv8(desc, q, kc, vc, ks, vs, table, i32(b.cu), i32(b.ctxs), None, out, window, sinks)
+        outs.append(out)
+    assert outs[0].isfinite().all() and torch.equal(*outs)
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+def test_a_nan_query_stays_in_its_row(rows):
+    """NaN in one row and head of q: that output is NaN, every other one is as without it."""
+    d, nh, nkv = dev(), 8, 2
+    b = ref.batch([rows, rows], [700, rows + 40], rows)
+    g = torch.Generator(device=d).manual_seed(rows)
+    q = torch.randn((b.total, nh * HD), generator=g, device=d).to(torch.bfloat16)
+    cache = ref.random_cache(b.blocks, nkv, 5, d)
+    desc, outs = make_desc(b, nh, nkv), []
+    for bad in (False, True):
+        if bad:
+            q[1, 5 * HD + 7] = math.nan
+        out = torch.empty((b.total, nh * HD), dtype=torch.bfloat16, device=d)
+        ck.paged_attention_verify_kv8(desc, q, *cache, table_of(b), i32(b.cu), i32(b.ctxs), None, out)
+        outs.append(out)
+    assert outs[1][1, 5 * HD:6 * HD].isnan().all()
+    outs[1][1, 5 * HD:6 * HD] = outs[0][1, 5 * HD:6 * HD]
+    # a NaN score changes the moment at which its group's reference rises, not the values beyond rounding:
+    # two orders of the same sum differ by less than a bf16 unit of the largest output
+    diff = (outs[0].float() - outs[1].float()).abs().max()
+    assert diff <= outs[0].float().abs().max() * 2.0 ** -7
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+def test_sequences_may_share_pages(rows):
+    """A common prefix held once: the same page ids in several tables."""
+    d, nh, nkv, shared = dev(), 16, 8, 20
+    b = ref.batch([rows] * 3, [shared * PAGE + rows + n for n in (0, 40, 700)], rows)
+    for t in b.tables[1:]:
+        t[:shared] = b.tables[0][:shared]
+    g = torch.Generator(device=d).manual_seed(rows)
+    q = torch.randn((b.total, nh * HD), generator=g, device=d).to(torch.bfloat16)
+    cache = ref.random_cache(b.blocks, nkv, 6, d)
+    out = torch.empty((b.total, nh * HD), dtype=torch.bfloat16, device=d)
+    ck.paged_attention_verify_kv8(make_desc(b, nh, nkv), q, *cache, table_of(b), i32(b.cu), i32(b.ctxs), None, out)
+    want, pv, sb = ref.attention(q, *cache, b.tables, b.q_lens, b.ctxs, nkv)
+    ref.assert_attention(out, want, pv, sb, max(b.ctxs))
+
+
 @pytest.mark.parametrize("rows", [2, 150])
 @pytest.mark.parametrize("what", ["wide", "zero", "odd", "huge"])
 def test_scales(rows, what):
