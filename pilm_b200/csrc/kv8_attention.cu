@@ -144,35 +144,31 @@ __device__ __forceinline__ void finish4(__nv_bfloat16 *out, const __nv_bfloat16 
 }
 
 // ---------------------------------------------------------------------------------
-// Geometry shared by the kernels.  A batch's rows are cut into groups: group (b, rg) holds the
-// rows rho in [rg * rpg, (rg + 1) * rpg) of sequence b, rho = j * gsz + g for query row j and
-// head g of a KV head's group.  A group's keys are a list of nv pages: the first n_sink pages
-// of the sequence, then those from lo_page on.
+// Geometry shared by the kernels.  rho = j * gsz + g numbers a sequence's rows, for query row j and
+// head g of a KV head's group.  The token kernel takes a sequence's rows together; the keys that
+// they see are a list of nv pages: the first n_sink pages of the sequence, then those from lo_page
+// on.
 // ---------------------------------------------------------------------------------
 struct Geometry {
     const int32_t *cu_q, *ctx;
-    int gsz, rpg, rgs;  // query heads per KV head, rows per group, groups per sequence
+    int gsz;            // query heads per KV head
     int window, sinks;  // window 0: none
 };
 struct Group {
-    int q0, rows, p0, ctx;      // first row, rows (rho) of the sequence, position of row j = 0
-    int rho0, rho1;             // this group's rows
+    int q0, rows, p0, ctx;  // first row, rows (rho) of the sequence, position of row j = 0
     int n_sink, lo_page, nv;
 };
 
-__device__ __forceinline__ Group group_of(const Geometry &g, int vs) {
+__device__ __forceinline__ Group group_of(const Geometry &g, int rpg, int b) {  // rpg: rows at most
     Group r;
-    const int b = vs / g.rgs, rg = vs % g.rgs;
     r.q0 = g.cu_q[b];
     const int q_len = g.cu_q[b + 1] - r.q0;
     r.ctx = g.ctx[b];
-    r.rows = q_len * g.gsz;
+    r.rows = min(q_len * g.gsz, rpg);
     r.p0 = r.ctx - q_len;
-    r.rho0 = rg * g.rpg;
-    r.rho1 = min(r.rows, r.rho0 + g.rpg);
     r.n_sink = r.lo_page = r.nv = 0;
-    if (r.rho0 >= r.rho1) return r;
-    const int pmin = r.p0 + r.rho0 / g.gsz, pmax = r.p0 + (r.rho1 - 1) / g.gsz;
+    if (r.rows <= 0) return r;
+    const int pmin = r.p0, pmax = r.p0 + (r.rows - 1) / g.gsz;
     if (pmax < 0) return r;
     const int end = (pmax >> 4) + 1;
     if (g.window > 0) {
@@ -238,14 +234,14 @@ struct TokParams {
     float *part;      // [head groups][G][2][hg * rpg][kRec]
     int *prefix_out;  // [groups + 1]: blocks before each group, for the merge
     int nh, nkv, max_blocks, num_blocks;
-    int groups, hg, ch, kw, pps, stages, G;
+    int groups, hg, ch, kw, pps, rpg, stages, G;  // groups: sequences; rpg = 16 ch rows of each
     int whole;  // a CTA per group (and head group) instead of equal shares of all pages
 };
 
 // Rows of a group that sees no key.
 __device__ void zero_rows(const TokParams &p, const Group &g, int head0, int heads) {
-    for (int i = threadIdx.x; i < (g.rho1 - g.rho0) * heads * (kHD / 8); i += blockDim.x) {
-        const int d = i % (kHD / 8), h = i / (kHD / 8) % heads, rho = g.rho0 + i / (kHD / 8) / heads;
+    for (int i = threadIdx.x; i < g.rows * heads * (kHD / 8); i += blockDim.x) {
+        const int d = i % (kHD / 8), h = i / (kHD / 8) % heads, rho = i / (kHD / 8) / heads;
         if (head0 + h >= p.nkv) continue;
         const size_t row = (size_t)(g.q0 + rho / p.geo.gsz) * p.nh + (head0 + h) * p.geo.gsz + rho % p.geo.gsz;
         *reinterpret_cast<uint4 *>(p.out + row * kHD + 8 * d) = make_uint4(0u, 0u, 0u, 0u);
@@ -285,7 +281,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     int x0, x1;  // this CTA's blocks
     int v_first;       // the group of block x0
     if (p.whole) {     // (s_prefix: only the CTA's own group, from 0)
-        const Group own = group_of(p.geo, cta);
+        const Group own = group_of(p.geo, p.rpg, cta);
         v_first = cta;
         x0 = 0, x1 = (own.nv + p.pps - 1) / p.pps;
         __syncthreads();
@@ -294,35 +290,35 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             return;
         }
     } else {
-    if (warp == 0) {  // blocks before each group
-        int carry = 0;
-        if (lane == 0) s_prefix[0] = 0;
-        for (int v0 = 0; v0 < p.groups; v0 += 32) {
-            const int v = v0 + lane;
-            int n = v < p.groups ? (group_of(p.geo, v).nv + p.pps - 1) / p.pps : 0;
+        if (warp == 0) {  // blocks before each group
+            int carry = 0;
+            if (lane == 0) s_prefix[0] = 0;
+            for (int v0 = 0; v0 < p.groups; v0 += 32) {
+                const int v = v0 + lane;
+                int n = v < p.groups ? (group_of(p.geo, p.rpg, v).nv + p.pps - 1) / p.pps : 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, n, o);
-                if (lane >= o) n += up;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, n, o);
+                    if (lane >= o) n += up;
+                }
+                if (v < p.groups) s_prefix[v + 1] = carry + n;
+                carry += __shfl_sync(0xffffffffu, n, 31);
             }
-            if (v < p.groups) s_prefix[v + 1] = carry + n;
-            carry += __shfl_sync(0xffffffffu, n, 31);
         }
-    }
-    __syncthreads();
-    if (cta == 0 && blockIdx.y == 0 && p.groups > kMergeScan)
-        for (int v = threadIdx.x; v <= p.groups; v += blockDim.x) p.prefix_out[v] = s_prefix[v];
-    for (int v = cta; v < p.groups; v += p.G)
-        if (s_prefix[v] == s_prefix[v + 1]) zero_rows(p, group_of(p.geo, v), head0, p.hg);
-    const int T = s_prefix[p.groups];
-    x0 = share_of(cta, T, p.G), x1 = share_of(cta + 1, T, p.G);
-    if (x0 >= x1) return;
-    int lo = 0, hi = p.groups - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
-    }
-    v_first = lo;
+        __syncthreads();
+        if (cta == 0 && blockIdx.y == 0 && p.groups > kMergeScan)
+            for (int v = threadIdx.x; v <= p.groups; v += blockDim.x) p.prefix_out[v] = s_prefix[v];
+        for (int v = cta; v < p.groups; v += p.G)
+            if (s_prefix[v] == s_prefix[v + 1]) zero_rows(p, group_of(p.geo, p.rpg, v), head0, p.hg);
+        const int T = s_prefix[p.groups];
+        x0 = share_of(cta, T, p.G), x1 = share_of(cta + 1, T, p.G);
+        if (x0 >= x1) return;
+        int lo = 0, hi = p.groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
+        }
+        v_first = lo;
     }
     auto start = [&](int v) { return p.whole ? (v == v_first ? 0 : x1) : s_prefix[v]; };
     const uint32_t ring = smem_u32(smem);
@@ -332,17 +328,17 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp > kTokWarps) return;
         int v = v_first, issued = 0;
-        Group g = group_of(p.geo, v);
+        Group g = group_of(p.geo, p.rpg, v);
         bool ok = true;
         // a block's page ids are fetched one block ahead (lane i: page i of the block)
         auto fetch = [&](int x, int &vv, Group &gg) {
             if (x >= x1) return -1;
-            while (x >= start(vv + 1)) gg = group_of(p.geo, ++vv);
+            while (x >= start(vv + 1)) gg = group_of(p.geo, p.rpg, ++vv);
             const int vp = (x - start(vv)) * p.pps + lane;
             int blk = -1;
             if (lane < p.pps && vp < gg.nv) {
                 const int pg = page_of(gg, vp);
-                if (pg < p.max_blocks) blk = p.block_table[(size_t)(vv / p.geo.rgs) * p.max_blocks + pg];
+                if (pg < p.max_blocks) blk = p.block_table[(size_t)vv * p.max_blocks + pg];
                 if (blk < 0 || blk >= p.num_blocks) blk = -1;
             }
             return blk;
@@ -416,13 +412,13 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     int segs = 0;
     for (int x = x0; x < x1 && ok; ++segs) {
         while (x >= start(v + 1)) ++v;
-        const Group g = group_of(p.geo, v);
+        const Group g = group_of(p.geo, p.rpg, v);
         const int seg1 = min(x1, start(v + 1));
         const bool whole = x == start(v) && seg1 == start(v + 1);
         const int slot = x == x0 ? 0 : 1;
-        const int tile0 = g.rho0 + 16 * c_of;
-        const bool active = head_ok && tile0 < g.rho1;
-        const int tile1 = min(g.rho1, tile0 + 16);
+        const int tile0 = 16 * c_of;
+        const bool active = head_ok && tile0 < g.rows;
+        const int tile1 = min(g.rows, tile0 + 16);
 
         // queries in f16 as q * 2^k, the largest magnitude of the row in [2^14, 2^15): exact for bf16
         // elements down to 2^-28 of the largest; 2^-k goes into the row's score factor
@@ -694,8 +690,8 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                     if (whole) {
                         finish4(p.out, p.gate, ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD + 4 * lane, O, f);
                     } else {
-                        float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.geo.rpg +
-                                               (size_t)h_of * p.geo.rpg + (rho - g.rho0)) * kRec;
+                        float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.rpg +
+                                               (size_t)h_of * p.rpg + rho) * kRec;
                         *reinterpret_cast<float4 *>(rec + 4 * lane) = make_float4(O[0] * f, O[1] * f, O[2] * f, O[3] * f);
                         if (lane == 0) rec[kHD] = M, rec[kHD + 1] = L;
                     }
@@ -726,8 +722,8 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                         store8(p.out + at, e);
                     }
             } else {
-                float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.geo.rpg +
-                                       (size_t)h_of * p.geo.rpg + (rho - g.rho0)) * kRec;
+                float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.rpg +
+                                       (size_t)h_of * p.rpg + rho) * kRec;
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -757,18 +753,17 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
     const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0;
     const bool in = head < p.nh && j < q_len;
     const int kvh = in ? head / p.geo.gsz : 0, rho = j * p.geo.gsz + (in ? head % p.geo.gsz : 0);
-    const int v = b * p.geo.rgs + rho / p.geo.rpg;
     int T = 0, P0 = 0, P1 = 0;
     if (p.groups <= kMergeScan) {
         for (int v0 = 0; v0 < p.groups; v0 += 32) {
-            const int x = v0 + lane, n = x < p.groups ? (group_of(p.geo, x).nv + p.pps - 1) / p.pps : 0;
+            const int x = v0 + lane, n = x < p.groups ? (group_of(p.geo, p.rpg, x).nv + p.pps - 1) / p.pps : 0;
             T += __reduce_add_sync(0xffffffffu, n);
-            P0 += __reduce_add_sync(0xffffffffu, x < v ? n : 0);
-            P1 += __reduce_add_sync(0xffffffffu, x <= v ? n : 0);
+            P0 += __reduce_add_sync(0xffffffffu, x < b ? n : 0);
+            P1 += __reduce_add_sync(0xffffffffu, x <= b ? n : 0);
         }
     } else {
         pdl_wait();
-        T = p.prefix_out[p.groups], P0 = p.prefix_out[v], P1 = p.prefix_out[v + 1];
+        T = p.prefix_out[p.groups], P0 = p.prefix_out[b], P1 = p.prefix_out[b + 1];
     }
     int c0 = 0, c1 = -1;
     if (in && P1 > P0) {
@@ -777,9 +772,9 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
     }
     pdl_wait();
     const bool cut = c1 > c0;  // else its one CTA wrote the output
-    const size_t rows = (size_t)p.hg * p.geo.rpg;
+    const size_t rows = (size_t)p.hg * p.rpg;
     const float *base = p.part + ((size_t)(kvh / p.hg) * p.G * 2) * rows * kRec +
-                        ((size_t)(kvh % p.hg) * p.geo.rpg + rho % p.geo.rpg) * kRec;
+                        ((size_t)(kvh % p.hg) * p.rpg + rho) * kRec;
     float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
     if (cut)
         for (int cb = c0 + sub * U; cb <= c1; cb += wpi * U) {
@@ -875,14 +870,14 @@ constexpr size_t kChSmem = kChSmemV + 2 * (size_t)kChOperand + 1024;
 constexpr int kChScales = 4;  // blocks whose scales are kept: the softmax may be two behind the copies
 
 struct ChunkParams {
-    Geometry geo;  // rpg = kChRows
+    Geometry geo;
     const __nv_bfloat16 *q, *gate;
     const uint8_t *kc, *vc;
     const float *ks, *vs;
     const int32_t *block_table;
     __nv_bfloat16 *out;
     float *part;  // [splits][total_q][nh][kRec], when splits > 1
-    int nh, nkv, max_blocks, num_blocks, total_q, splits;
+    int nh, nkv, max_blocks, num_blocks, total_q, rgs, splits;  // rgs: groups of kChRows rows per sequence
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -1004,7 +999,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     pdl_wait();
 
     // the last positions see the most keys: their groups first
-    const int per = (int)gridDim.x / p.geo.rgs, rg = p.geo.rgs - 1 - blockIdx.x / per, in_rg = blockIdx.x % per;
+    const int per = (int)gridDim.x / p.rgs, rg = p.rgs - 1 - blockIdx.x / per, in_rg = blockIdx.x % per;
     const int split = in_rg % p.splits, kvh = in_rg / p.splits % p.nkv, b = in_rg / (p.splits * p.nkv);
     const int q0 = p.geo.cu_q[b], q_len = p.geo.cu_q[b + 1] - q0, ctx = p.geo.ctx[b];
     const int gsz = p.geo.gsz, p0 = ctx - q_len;
@@ -1433,7 +1428,7 @@ __global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int nu
 // Host side
 // ---------------------------------------------------------------------------------
 struct TokPlan {
-    int hg, ngroups, ch, kw, pps, rpg, rgs, G, whole, stages, seqs_per_launch;
+    int hg, ngroups, ch, kw, pps, G, whole, stages;
     size_t stage_bytes, smem, part_bytes, prefix_bytes;
 };
 
@@ -1443,16 +1438,13 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
     TokPlan t;
     const int nkv = (int)d->n_kv_heads, gsz = (int)(d->n_heads / d->n_kv_heads), sms = num_sms();
     const long long max_q = (long long)(d->max_q_len < 1 ? 1 : (d->max_q_len < d->total_q ? d->max_q_len : d->total_q));
-    const long long rows = max_q * gsz;
-    t.ch = (int)(rows > 16 * kTokWarps ? kTokWarps : (rows + 15) / 16);  // row tiles share the pages a CTA reads
-    t.rpg = 16 * t.ch;
-    t.rgs = (int)((rows + t.rpg - 1) / t.rpg);
+    t.ch = (int)(max_q * gsz + 15) / 16;  // 1 or 2 row tiles share the pages that a CTA reads
     long long keys = (long long)d->max_context;
     if (window > 0 && window < (1u << 30) && sinks < (1u << 30)) {
         const long long seen = (long long)window + (long long)sinks + max_q + 32;
         if (seen < keys) keys = seen;
     }
-    const long long pages = (keys + 15) / 16, groups = (long long)d->num_seqs * t.rgs;
+    const long long pages = (keys + 15) / 16, groups = (long long)d->num_seqs;
     auto shape = [&](int heads) {  // KV heads per CTA, the rest of the warps on different pages
         t.ngroups = (nkv + heads - 1) / heads;
         t.hg = (nkv + t.ngroups - 1) / t.ngroups;
@@ -1481,19 +1473,19 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
         }
         break;
     }
-    t.seqs_per_launch = t.rgs >= kTokGroups ? 1 : kTokGroups / t.rgs;
     t.stage_bytes = (size_t)t.pps * t.hg * 4096;
     const size_t join = t.kw > 1 && t.ch > 1 ? (size_t)t.hg * t.ch * t.kw * 16 * kHD * sizeof(float) : 0;
     t.stages = (int)((kTokSmem - join) / t.stage_bytes);
     if (t.stages > kTokStages) t.stages = kTokStages;
     t.smem = t.stages * t.stage_bytes + join + 1024;
-    t.part_bytes = t.whole ? 0 : (size_t)t.ngroups * t.G * 2 * t.hg * t.rpg * kRec * sizeof(float);
+    t.part_bytes = t.whole ? 0 : (size_t)t.ngroups * t.G * 2 * t.hg * 16 * t.ch * kRec * sizeof(float);
     t.prefix_bytes = (size_t)(kTokGroups + 4) * sizeof(int);
     return t;
 }
 
 struct ChunkPlan {
     int rgs, splits;
+    long long ctas;
     size_t part_bytes;
 };
 
@@ -1522,7 +1514,8 @@ bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks
     if (s > blocks / 3) s = blocks / 3;
     c.splits = (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
     c.part_bytes = c.splits > 1 ? (size_t)c.splits * d->total_q * d->n_heads * kRec * sizeof(float) : 0;
-    return ctas * c.splits <= 0x7fffffffLL;
+    c.ctas = ctas * c.splits;
+    return true;
 }
 
 int encode_pages(const uint8_t *kc, const uint8_t *vc, int nkv, int num_blocks, int hg, CUtensorMap (&maps)[2],
@@ -1592,10 +1585,10 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
     geo.sinks = (int)(sinks < cap ? sinks : cap);
     ChunkPlan c;
     if (plan_chunks(desc, window, sinks, c)) {
+        PILM_REQUIRE(c.ctas <= 0x7fffffffLL, ECPU_ERR_PARAM, "%s: too many rows", what);
         ChunkParams p;
         p.geo = geo;
-        p.geo.rpg = kChRows;
-        p.geo.rgs = c.rgs;
+        p.rgs = c.rgs;
         p.q = (const __nv_bfloat16 *)q;
         p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
         p.kc = k_cache;
@@ -1612,7 +1605,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.total_q = (int)desc->total_q;
         p.splits = c.splits;
         cudaFuncSetAttribute(kv8_attn_chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChSmem);
-        launch_pdl(kv8_attn_chunk, dim3((unsigned)(desc->num_seqs * c.rgs * c.splits * p.nkv)), dim3(kChThreads),
+        launch_pdl(kv8_attn_chunk, dim3((unsigned)c.ctas), dim3(kChThreads),
                    kChSmem, p);
         rc = check_launch(what);
         if (rc == ECPU_OK) rc = check_error(what);
@@ -1629,15 +1622,13 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
     rc = encode_pages(k_cache, v_cache, (int)desc->n_kv_heads, (int)desc->num_blocks, t.hg, maps, what);
     if (rc != ECPU_OK) return rc;
     cudaFuncSetAttribute(kv8_attn_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kTokSmem + 1024));
-    for (size_t b0 = 0; b0 < desc->num_seqs; b0 += (size_t)t.seqs_per_launch) {
-        const int seqs = (int)(desc->num_seqs - b0 < (size_t)t.seqs_per_launch ? desc->num_seqs - b0
-                                                                               : (size_t)t.seqs_per_launch);
+    for (size_t b0 = 0; b0 < desc->num_seqs; b0 += (size_t)kTokGroups) {
+        const int seqs = (int)(desc->num_seqs - b0 < (size_t)kTokGroups ? desc->num_seqs - b0 : (size_t)kTokGroups);
         TokParams p;
         p.geo = geo;
         p.geo.cu_q += b0;
         p.geo.ctx += b0;
-        p.geo.rpg = t.rpg;
-        p.geo.rgs = t.rgs;
+        p.rpg = 16 * t.ch;
         p.q = (const __nv_bfloat16 *)q;
         p.gate = desc->output_gate ? (const __nv_bfloat16 *)gate : nullptr;
         p.ks = k_scale;
@@ -1650,7 +1641,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.nkv = (int)desc->n_kv_heads;
         p.max_blocks = (int)desc->max_blocks_per_seq;
         p.num_blocks = (int)desc->num_blocks;
-        p.groups = seqs * t.rgs;
+        p.groups = seqs;
         p.hg = t.hg;
         p.ch = t.ch;
         p.kw = t.kw;
@@ -1670,7 +1661,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         // A group's partials lie in span CTAs at most.  As many warps share a row and head as load them
         // in one round (8 sequences of 5 rows over 4K keys: 38.0 us with 16 warps, 24.6 with 4); 16
         // with 10 loads each where one wave of blocks holds them all (8 rows over 8K: 20.2 against 21.1).
-        const int span = t.G / (seqs * t.rgs) + 2;
+        const int span = t.G / seqs + 2;
         const bool wide = span > 8 && (long long)max_q * p.nh * seqs <= num_sms();
         int wpi = wide ? 16 : 1;
         while (!wide && wpi < 8 && 8 * wpi < span) wpi *= 2;
