@@ -475,7 +475,7 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
             "unit": "GB/s",
             "frac": round(att_gbs / pk["hbm_gbs"], 4) if att_gbs else None,
             "traffic": traffic,
-            "traffic_source": cap["source"] if cap else None,
+            "traffic_source": cap["source"] if cap and traffic else None,
             "algorithmic_bytes_per_launch": att_bytes,
             "avg_launch_ms": round(att_ms, 5) if att_ms else None,
         },

@@ -514,8 +514,9 @@ int ekernel_qk_norm_rope_kv_append_kv8_splitk(const ekernel_paged_attn_desc_t *d
  *    output is 0.  Rows of `out` from cu_q[num_seqs] on are not written.
  *  - A block id outside [0, num_blocks) reads as a page of zeros.  Bytes past the context are
  *    read as nothing whatever they hold; NaN codes (0x7F, 0xFF) below it must not occur.
- *  - Scores, softmax and sums are fp32 (queries and keys multiply exactly); probabilities are
- *    rounded to f16 for the product with V; the output is rounded once, after the gate.
+ *  - Scores, softmax and sums are fp32.  Queries enter the product in f16 at a power of two of their
+ *    row's own (exact for elements down to 2^-28 of the row's largest), keys exactly; probabilities
+ *    are rounded to f16 for the product with V; the output is rounded once, after the gate.
  *  - workspace: at least ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks)
  *    bytes, 16-byte aligned, its contents undefined before and after.  The library allocates
  *    none of its own, so calls that may overlap on the GPU (other streams, other graphs) need

@@ -197,23 +197,31 @@ __device__ __forceinline__ int cta_of(int x, int T, int G) {
 }
 
 // ---------------------------------------------------------------------------------
-// Token kernel: decode and verify rows, bound by reading the cache.
+// Token kernel: calls of at most 32 rows per KV head (decode, verify), bound by reading the cache.
 //
-// One CTA per SM.  The groups' pages, in blocks of `pps`, form one list that the CTAs of a head
+// One CTA per SM.  The sequences' pages, in blocks of `pps`, form one list that the CTAs of a head
 // group share evenly: a producer warp streams whole blocks (K and V of `hg` KV heads) through a
 // TMA ring, and consumer warp (h, c, k) takes head h, row tile c (16 rows) and pages 2k, 2k + 1
-// of each block, so every byte is read from HBM once and 8 warps share the conversions.
+// of each block, so every byte is read from HBM once and 8 warps share the conversions.  A sequence
+// that a boundary cuts leaves partial sums for the merge kernel; with few sequences and short
+// contexts a CTA takes a whole sequence and there is nothing to merge.
 //
-// Per pair of pages a warp computes S = Q K8^T with mma.sync m16n8k32 on the codes as they are
-// (the queries split into two e4m3 parts), and O += P V8 with m16n8k16 on f16 (P needs f16's
-// range; V's codes are converted in registers as they leave shared memory).  Both products sum over an index whose order is free, and each order is chosen so that a thread's
-// operand is contiguous in the cache as it lies there: thread (g, c) = (lane / 4, lane % 4) holds
-// dims 32c .. 32c + 31 of a key for S, and dims 16g .. 16g + 15 of its four keys for O, where
-// four byte permutes pair the keys.  With the TMA's 128-byte swizzle all these 16-byte
-// shared-memory loads are free of bank conflicts.
+// Per pair of pages a warp computes S = Q K8^T and O += P V8 with mma.sync m16n8k16 on f16, the
+// codes converted in registers as they leave shared memory (e4m3 operands run no faster: sm_100 has
+// no e4m3 mma.sync of its own).  Both products sum over an index whose order is free, and each order
+// is chosen so that a thread's operand is contiguous in the cache as it lies there: thread (g, c) =
+// (lane / 4, lane % 4) holds dims 32c .. 32c + 31 of a key for S, and dims 16g .. 16g + 15 of its
+// four keys for O, where four byte permutes pair the keys.  With the TMA's 128-byte swizzle all these
+// 16-byte shared-memory loads are free of bank conflicts.
 //
 // The tcgen05 pipe does not fit these shapes: one token's rows (gsz = 4, say) would fill 4 of its
 // 128 rows.  mma.sync at 16 rows keeps up with HBM.
+//
+// Measured, in a captured graph: 96 verify rows over 32 x 8236 keys, 32 + 8 heads: 93.0 us with the
+// merge, 5.15 TB/s of cache, where the copy of as many bytes takes 74 us and this kernel with its
+// arithmetic left out 89 (sums of pages differ by up to a block of 0.8 us between the CTAs, and the
+// first bytes arrive 6 us after the start).  One row over 131071 keys 55.3 us, 4.86 TB/s; one row over 301
+// keys 9.1 us, a chain of loads (lengths -> page ids -> pages) and two products.
 // ---------------------------------------------------------------------------------
 constexpr int kTokWarps = 8;      // consumer warps at most
 // Three warpgroups: two of consumers, and one whose first warp is the producer.  Launched with
@@ -859,10 +867,19 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
 // exponent: p' = 2^(s f + c), c = bits - m + log2(vs / vref), one fma and one exp2 per score.
 // Register split of the 512 threads (128 each at launch, 65536): 184 for the softmax warps, 104 for
 // the converters, 40 for the issuer's group: 256 * 184 + 128 * 104 + 128 * 40 = 65536.
+//
+// Measured: two prompts of 4096 rows, 32 + 8 heads: 277 us, 731 TFLOP/s (the products alone at the
+// card's f16 rate: 118); 8192 rows through a 1024-key window 261 us.  A block of both tiles takes
+// 2.0 to 2.4 us, of which the tensor cores work 1.5 (an M = 128, N = 128 product takes 88 cycles
+// of the ideal 64) and the exponentials 1.04; a tile's next scores wait for its P to be used, as
+// TMEM is full.  A CTA's first scores come 6 us after its start, its last stores 4 us after the last P.
+// Measured and left out: 64-key blocks with two score buffers (349 us: N = 64 products cost nearly what N = 128
+// ones do, twice the hand-overs), 16 softmax warps (348), scores held in registers, and blocks that take over
+// the next group (355: the converters' loads in flight no longer fit their registers).
 // ---------------------------------------------------------------------------------
 constexpr int kChThreads = 512;
 constexpr int kChTile = 128, kChRows = 2 * kChTile;  // rows per tile and per CTA
-constexpr int kChKeys = 128;                         // keys per block
+constexpr int kChKeys = 128, kChPages = kChKeys / kKv8Page;  // keys and pages per block
 constexpr int kChHalf = kChKeys * 128;               // 64 dims of a 128-row f16 operand: 16 KB
 constexpr int kChOperand = 2 * kChHalf;              // 32 KB
 constexpr size_t kChSmemK = 2 * (size_t)kChOperand, kChSmemV = kChSmemK + 2 * (size_t)kChOperand;
@@ -1005,21 +1022,22 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     const int gsz = p.geo.gsz, p0 = ctx - q_len;
     const int rho0 = rg * kChRows, rho1 = min(q_len * gsz, rho0 + kChRows);
     const int tiles = rho1 - rho0 > kChTile ? 2 : (rho1 > rho0 ? 1 : 0);
-    // blocks of the group: n_sink from the first key on, then those from lo on
-    int n_sink = 0, lo = 0, nb = 0, first = 0;  // first: the page of the first key within a window
+    // the group's pages: n_sink from the sequence's first on, then those from lo_page on, nv in all;
+    // block j holds the pages 8 j .. 8 j + 7 of this list
+    int n_sink = 0, lo_page = 0, nv = 0;
     if (tiles > 0) {
         const int pmin = p0 + rho0 / gsz, pmax = p0 + (rho1 - 1) / gsz;
         if (pmax >= 0) {
             if (p.geo.window > 0) {
-                first = max(0, pmin - p.geo.window + 1) / kKv8Page * kKv8Page;
-                lo = first / kChKeys;
-                n_sink = min((p.geo.sinks + kChKeys - 1) / kChKeys, lo);
+                lo_page = max(0, pmin - p.geo.window + 1) / kKv8Page;
+                n_sink = min((p.geo.sinks + kKv8Page - 1) / kKv8Page, lo_page);
             }
-            nb = n_sink + pmax / kChKeys + 1 - lo;
+            nv = n_sink + pmax / kKv8Page + 1 - lo_page;
         }
     }
+    const int nb = (nv + kChPages - 1) / kChPages;
     const int j0 = (int)((long long)nb * split / p.splits), j1 = (int)((long long)nb * (split + 1) / p.splits);
-    auto key_of = [&](int j) { return (j < n_sink ? j : j - n_sink + lo) * kChKeys; };
+    auto key_of = [&](int i) { return (i < n_sink ? i : i - n_sink + lo_page) * kKv8Page; };  // page i's first
     // a wait of the whole warp; false once any lane gave up
     auto wait = [&](uint64_t *m, uint32_t parity) {
         const bool ok = __all_sync(0xffffffffu, mbar_wait(m, parity, &s_abort));
@@ -1094,15 +1112,12 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         // ---- converters: thread (row, ch) takes 16 codes of token `row` of each of a block's pages ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int tid = threadIdx.x - 256, row = tid >> 3, ch = tid & 7;
-        const int32_t *bt = p.block_table + (size_t)b * p.max_blocks;
         // page ids of block j: lane i holds page i's
         auto fetch_ids = [&](int j) {
             int blk = -1;
             if (j < j1 && lane < 8) {
-                const int pg = key_of(j) / kKv8Page + lane;
-                // past the context, or wholly outside the rows' windows (its id may be another's by now)
-                if (pg < p.max_blocks && pg * kKv8Page < ctx && (pg * kKv8Page >= first || pg * kKv8Page < p.geo.sinks))
-                    blk = bt[pg];
+                const int i = j * kChPages + lane, pg = key_of(i) / kKv8Page;
+                if (i < nv && pg < p.max_blocks && pg * kKv8Page < ctx) blk = p.block_table[(size_t)b * p.max_blocks + pg];
                 if (blk < 0 || blk >= p.num_blocks) blk = -1;
             }
             return blk;
@@ -1121,13 +1136,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         const int c0 = 2 * (ch & 3) + (ch >> 2), c1 = c0 ^ 1;
         const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((c0 ^ (row & 7)) << 4);
         const uint32_t dst1 = (ch >> 2) * kChHalf + row * 128 + ((c1 ^ (row & 7)) << 4);
-        auto convert = [&](uint32_t at, int j, uint32_t valid, const uint4 (&r)[8]) {
-            const bool whole = valid == 0xffu && key_of(j) + kChKeys <= ctx;
-            const int keys = ctx - key_of(j) - row;  // keys past the context, pages without a valid id
+        // live: bit i: this thread's token of page i counts (the page has a valid id, the token is one
+        // of the context's)
+        auto convert = [&](uint32_t at, uint32_t live, const uint4 (&r)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-                if (!whole && !(((valid >> i) & 1u) && 16 * i < keys)) w[0] = w[1] = w[2] = w[3] = 0u;
+                if (live != 0xffu && !((live >> i) & 1u)) w[0] = w[1] = w[2] = w[3] = 0u;
                 const bool sw = ch >> 2;  // the chunk written first: the second one's lanes swap the words
                 const uint32_t a0 = sw ? w[2] : w[0], a1 = sw ? w[3] : w[1], b0 = sw ? w[0] : w[2], b1 = sw ? w[1] : w[3];
                 const uint32_t x[4] = {e4m3x2_to_f16x2(a0), e4m3x2hi_to_f16x2(a0), e4m3x2_to_f16x2(a1), e4m3x2hi_to_f16x2(a1)};
@@ -1152,7 +1167,10 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             const uint32_t parity = (uint32_t)((n >> 1) - 1) & 1u;
             // scales of the block's pages (warp 8: lanes 0..7 K, 8..15 V); zero without a valid id
             float sc = 0.f;
-            const uint32_t valid = __ballot_sync(0xffffffffu, ids >= 0);
+            const bool cut = key_of(j * kChPages + lane) + kKv8Page > ctx;  // the context ends in the page
+            uint32_t live = __ballot_sync(0xffffffffu, ids >= 0 && !cut);
+            const uint32_t last = __ballot_sync(0xffffffffu, ids >= 0 && cut);
+            if (row < (ctx & (kKv8Page - 1))) live |= last;
             if (warp == 8) {
                 const int blk = __shfl_sync(0xffffffffu, ids, lane & 7);
                 sc = (lane < 8 ? p.ks : p.vs)[(size_t)max(blk, 0) * p.nkv + kvh];
@@ -1162,12 +1180,12 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             if (n >= 2) ok = wait(&bar.k_empty[st], parity);
             if (!ok) break;
             if (warp == 8 && lane < 16) s_scale[n % kChScales][lane >> 3][lane & 7] = sc;
-            convert(base + (uint32_t)kChSmemK + st * kChOperand, j, valid, kr);
+            convert(base + (uint32_t)kChSmemK + st * kChOperand, live, kr);
             publish(&bar.k_full[st]);
             fetch(p.kc, next, kr);
             if (n >= 2) ok = wait(&bar.v_empty[st], parity);
             if (!ok) break;
-            convert(base + (uint32_t)kChSmemV + st * kChOperand, j, valid, vr);
+            convert(base + (uint32_t)kChSmemV + st * kChOperand, live, vr);
             publish(&bar.v_full[st]);
             fetch(p.vc, next, vr);
             ids = next;
@@ -1216,9 +1234,15 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         float m = -INFINITY, l = 0.f, vref = 0.f, inv_vref = 0.f;
         bool ok = true;
         if (t < tiles) {
-            // positions of the warp's rows: blocks that all of them see whole need no mask
+            // positions of the warp's rows: pages [plain0, plain1) of the list, which all of them see
+            // whole, need no mask
             const int w0 = rho0 + t * kChTile + (warp & 3) * 32, w1 = min(rho1, w0 + 32) - 1;
             const int pmin = p0 + w0 / gsz, pmax = p0 + (w1 >= w0 ? w1 : w0) / gsz;
+            int plain0 = 0, plain1 = max(pmin + 1, 0) / kKv8Page;
+            if (p.geo.window > 0) {
+                plain0 = n_sink + max(0, (max(0, pmax - p.geo.window + 1) + kKv8Page - 1) / kKv8Page - lo_page);
+                plain1 += n_sink - lo_page;
+            }
             const uint32_t s_at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 128 * t, o_at = s_at + 256;
             for (int j = j0, n = 0; j < j1; ++j, ++n) {
                 ok = wait(&bar.s_full[t], (uint32_t)n & 1u);
@@ -1230,21 +1254,16 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i], vtop = fmaxf(vtop, c2[i]);
                 }
-                const int key0 = key_of(j);
-                auto seen_whole = [&](int k0, int keys) {  // by all rows of the warp
-                    return k0 + keys - 1 <= pmin &&
-                           (p.geo.window == 0 || k0 > pmax - p.geo.window || k0 + keys - 1 < p.geo.sinks);
-                };
-                const bool plain = seen_whole(key0, kChKeys);
+                const bool plain = j * kChPages >= plain0 && (j + 1) * kChPages <= plain1;
                 if (!plain) {
                     // in pages that some row does not see whole, which at 128 keys a block are few, the
                     // others' scores become -inf, which must not meet a factor of 0 (with the least
                     // normal number in its place a product is still nothing beside the exponents)
 #pragma unroll 1
                     for (int i = 0; i < 8; ++i) {
-                        const int k0 = key0 + 16 * i;
-                        if (seen_whole(k0, 16)) continue;
-                        uint32_t s[16], see = low16(qp + 1 - k0);
+                        const int at = j * kChPages + i, k0 = key_of(at);
+                        if (at >= plain0 && at < plain1) continue;
+                        uint32_t s[16], see = at < nv ? low16(qp + 1 - k0) : 0u;
                         if (p.geo.window) see &= ~low16(qp - p.geo.window + 1 - k0) | low16(p.geo.sinks - k0);
                         tc_ld16(s_at + 16 * i, s);
                         tc_ld_wait();
@@ -1459,8 +1478,9 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
     t.whole = 0;
     t.G = (int)(blocks < 1 ? 1 : (blocks < per ? blocks : per));
     const long long share = (blocks + t.G - 1) / t.G;
-    // Or a CTA for each group and as few heads as the SMs allow: no partials, no second launch, whose
-    // time is that of about four blocks (measured: 3 us, 0.8 us a block).
+    // Or a CTA for each sequence and as few heads as the SMs allow: no partials, no second launch, whose
+    // time is that of about four blocks (measured: 3 us, 0.8 us a block; one row over 301 keys 14.2 us
+    // with shares, 9.1 whole; 8 sequences in a 100-key window 18.7 and 7.7).
     for (int heads = 1; heads <= kTokWarps / t.ch; heads *= 2) {
         if (groups * ((nkv + heads - 1) / heads) > sms) continue;
         const TokPlan shares = t;
