@@ -1111,7 +1111,9 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     } else if (warp >= 8) {
         // ---- converters: thread (row, ch) takes 16 codes of token `row` of each of a block's pages ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        const int tid = threadIdx.x - 256, row = tid >> 3, ch = tid & 7;
+        // Eight lanes (a phase of 16-byte accesses) have one half of two neighbouring rows, whose swizzle
+        // puts their chunks on all banks.
+        const int row = 4 * (warp - 8) + (lane >> 2 & 1) + 2 * (lane >> 4), ch = (lane & 3) | (lane >> 1 & 4);
         // page ids of block j: lane i holds page i's
         auto fetch_ids = [&](int j) {
             int blk = -1;
@@ -1131,11 +1133,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                 r[i] = ldg_nc_v4(cache + (((size_t)blk * kKv8Page + row) * p.nkv + kvh) * kHD + 16 * ch);
             }
         };
-        // dims 16 ch ..: two 16-byte chunks of the half ch / 4.  The lanes of the second half write
-        // their odd chunk first, so that eight lanes cover all banks.
-        const int c0 = 2 * (ch & 3) + (ch >> 2), c1 = c0 ^ 1;
-        const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((c0 ^ (row & 7)) << 4);
-        const uint32_t dst1 = (ch >> 2) * kChHalf + row * 128 + ((c1 ^ (row & 7)) << 4);
+        // dims 16 ch ..: two 16-byte chunks of the half ch / 4
+        const uint32_t dst0 = (ch >> 2) * kChHalf + row * 128 + ((2 * (ch & 3) ^ (row & 7)) << 4), dst1 = dst0 ^ 16u;
         // live: bit i: this thread's token of page i counts (the page has a valid id, the token is one
         // of the context's)
         auto convert = [&](uint32_t at, uint32_t live, const uint4 (&r)[8]) {
@@ -1143,10 +1142,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             for (int i = 0; i < 8; ++i) {
                 uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
                 if (live != 0xffu && !((live >> i) & 1u)) w[0] = w[1] = w[2] = w[3] = 0u;
-                const bool sw = ch >> 2;  // the chunk written first: the second one's lanes swap the words
-                const uint32_t a0 = sw ? w[2] : w[0], a1 = sw ? w[3] : w[1], b0 = sw ? w[0] : w[2], b1 = sw ? w[1] : w[3];
-                const uint32_t x[4] = {e4m3x2_to_f16x2(a0), e4m3x2hi_to_f16x2(a0), e4m3x2_to_f16x2(a1), e4m3x2hi_to_f16x2(a1)};
-                const uint32_t y[4] = {e4m3x2_to_f16x2(b0), e4m3x2hi_to_f16x2(b0), e4m3x2_to_f16x2(b1), e4m3x2hi_to_f16x2(b1)};
+                const uint32_t x[4] = {e4m3x2_to_f16x2(w[0]), e4m3x2hi_to_f16x2(w[0]), e4m3x2_to_f16x2(w[1]), e4m3x2hi_to_f16x2(w[1])};
+                const uint32_t y[4] = {e4m3x2_to_f16x2(w[2]), e4m3x2hi_to_f16x2(w[2]), e4m3x2_to_f16x2(w[3]), e4m3x2hi_to_f16x2(w[3])};
                 sts128(at + i * 2048 + dst0, x);
                 sts128(at + i * 2048 + dst1, y);
             }
