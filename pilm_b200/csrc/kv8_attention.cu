@@ -854,8 +854,9 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
 // ---------------------------------------------------------------------------------
 // Chunk kernel: prompts and other calls with many rows per KV head, bound by the tensor cores.
 //
-// A CTA owns 256 rows (two tiles of 128) of one KV head of one sequence and a range of its
-// 128-key blocks.  Four converter warps read a block's codes from the cache, write them to shared
+// A CTA owns 256 rows (two tiles of 128) of one KV head of one sequence and a share of the pages that
+// they see, in blocks of eight (128 keys): with a window, the sinks' pages and the window's follow
+// one another in a block.  Four converter warps read a block's codes from the cache, write them to shared
 // memory as f16 (K and V each into two 32 KB stages; the code-to-f16 step is shared by both tiles),
 // and one thread issues, per block and tile,
 //   S = Q K8^T    8 x tcgen05.mma M=128 N=128 K=16 (kind::f16), both operands in shared memory
@@ -865,17 +866,19 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
 // softmax runs the tensor cores work on the other tile.  The softmax takes the row maximum page by
 // page on the raw products (a page's scale is one factor) and folds the page's V scale into the
 // exponent: p' = 2^(s f + c), c = bits - m + log2(vs / vref), one fma and one exp2 per score.
-// Register split of the 512 threads (128 each at launch, 65536): 184 for the softmax warps, 104 for
-// the converters, 40 for the issuer's group: 256 * 184 + 128 * 104 + 128 * 40 = 65536.
+// Register split of the 512 threads (128 each at launch, 65536): 176 for the softmax warps, 120 for
+// the converters, 40 for the issuer's group: 256 * 176 + 128 * 120 + 128 * 40 = 65536.  (With fewer the
+// converters spill, and a spilled load in flight waits for itself.)
 //
-// Measured: two prompts of 4096 rows, 32 + 8 heads: 277 us, 731 TFLOP/s (the products alone at the
-// card's f16 rate: 118); 8192 rows through a 1024-key window 261 us.  A block of both tiles takes
-// 2.0 to 2.4 us, of which the tensor cores work 1.5 (an M = 128, N = 128 product takes 88 cycles
-// of the ideal 64) and the exponentials 1.04; a tile's next scores wait for its P to be used, as
-// TMEM is full.  A CTA's first scores come 6 us after its start, its last stores 4 us after the last P.
+// Measured: two prompts of 4096 rows, 32 + 8 heads: 275 us, 737 TFLOP/s (the products alone at the
+// card's f16 rate: 118); 8192 rows through a 1024-key window with 4 sinks 231 us, 560 TFLOP/s.  A
+// block of both tiles takes 2.0 to 2.4 us, of which the tensor cores work 1.5 (an M = 128, N = 128
+// product takes 88 cycles of the ideal 64) and the exponentials 1.04; a tile's next scores wait for its
+// P to be used, as TMEM is full.  A CTA's first scores come 6 us after its start, its last stores 4 us
+// after the last P.
 // Measured and left out: 64-key blocks with two score buffers (349 us: N = 64 products cost nearly what N = 128
 // ones do, twice the hand-overs), 16 softmax warps (348), scores held in registers, and blocks that take over
-// the next group (355: the converters' loads in flight no longer fit their registers).
+// the next group as they finish (355: more registers than there are).
 // ---------------------------------------------------------------------------------
 constexpr int kChThreads = 512;
 constexpr int kChTile = 128, kChRows = 2 * kChTile;  // rows per tile and per CTA
@@ -976,7 +979,7 @@ __device__ __forceinline__ float max16(const uint32_t *s) {
     return fmaxf(max3(a, b, c), d);
 }
 struct __align__(8) ChunkBars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drain;
 };
 
 // grid: (sequences x groups x splits, n_kv)
@@ -999,8 +1002,9 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i][0], 4);
             mbar_init(&bar.p_full[i][1], 4);
+            mbar_init(&bar.o_done[i], 1);
         }
-        mbar_init(&bar.o_done, 1);
+        mbar_init(&bar.drain, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -1096,21 +1100,22 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                             tc_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, va + k * (2048 >> 4),
                                       idesc_pv, n > 0 || k > 0 ? 1u : 0u);
                         if (t == tiles - 1) tc_commit(&bar.v_empty[n & 1]);
+                        if (n + 1 == total) tc_commit(&bar.o_done[t]);
                     }
                     __syncwarp();
                     if (n + 1 < total) issue_s(t, n + 1);  // after PV: S lies over P
                 }
             }
             // everything issued has completed (also when a wait gave up)
-            if (lane == 0) tc_commit(&bar.o_done);
+            if (lane == 0) tc_commit(&bar.drain);
             __syncwarp();
-            mbar_wait(&bar.o_done, 0, nullptr);
+            mbar_wait(&bar.drain, 0, nullptr);
             if (!ok && lane == 0) atomicExch(&g_kv8_error, 1);
             __syncwarp();
         }
     } else if (warp >= 8) {
         // ---- converters: thread (row, ch) takes 16 codes of token `row` of each of a block's pages ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
         // Eight lanes (a phase of 16-byte accesses) have one half of two neighbouring rows, whose swizzle
         // puts their chunks on all banks.
         const int row = 4 * (warp - 8) + (lane >> 2 & 1) + 2 * (lane >> 4), ch = (lane & 3) | (lane >> 1 & 4);
@@ -1189,7 +1194,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         }
     } else {
         // ---- softmax: thread = row ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int t = warp >> 2, r = threadIdx.x & 127;
         const int rho = rho0 + t * kChTile + r;
         const bool in = rho < rho1;
@@ -1352,7 +1357,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                     }
                 }
             }
-            if (ok && j0 < j1) ok = wait(&bar.o_done, 0);
+            if (ok && j0 < j1) ok = wait(&bar.o_done[t], 0);
             if (ok) {
                 tc_fence_after();
                 const float f = l > 0.f ? __fdiv_rn(vref, l) : 0.f;
