@@ -220,8 +220,8 @@ __device__ __forceinline__ int cta_of(int x, int T, int G) {
 // Measured, in a captured graph: 96 verify rows over 32 x 8236 keys, 32 + 8 heads: 93.0 us with the
 // merge, 5.15 TB/s of cache, where the copy of as many bytes takes 74 us and this kernel with its
 // arithmetic left out 89 (sums of pages differ by up to a block of 0.8 us between the CTAs, and the
-// first bytes arrive 6 us after the start).  One row over 131071 keys 55.3 us, 4.86 TB/s; one row over 301
-// keys 9.1 us, a chain of loads (lengths -> page ids -> pages) and two products.
+// first bytes arrive 5 us after the start).  One row over 131071 keys 54.8 us, 4.9 TB/s; one row over 301
+// keys 8.2 us, a chain of loads (lengths and page ids -> pages), two rounds of products and a join.
 // ---------------------------------------------------------------------------------
 constexpr int kTokWarps = 8;      // consumer warps at most
 // Three warpgroups: two of consumers, and one whose first warp is the producer.  Launched with
@@ -288,8 +288,12 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     pdl_trigger();
     int x0, x1;  // this CTA's blocks
     int v_first;       // the group of block x0
+    Group own;         // and its geometry
+    int early = -1;    // the producer's first page ids, where they can be asked for beside the lengths
     if (p.whole) {     // (s_prefix: only the CTA's own group, from 0)
-        const Group own = group_of(p.geo, p.rpg, cta);
+        if (warp == kTokWarps && p.geo.window == 0 && lane < min(p.pps, p.max_blocks))
+            early = p.block_table[(size_t)cta * p.max_blocks + lane];
+        own = group_of(p.geo, p.rpg, cta);
         v_first = cta;
         x0 = 0, x1 = (own.nv + p.pps - 1) / p.pps;
         __syncthreads();
@@ -327,6 +331,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             if (s_prefix[mid] <= x0) lo = mid; else hi = mid - 1;
         }
         v_first = lo;
+        own = group_of(p.geo, p.rpg, v_first);
     }
     auto start = [&](int v) { return p.whole ? (v == v_first ? 0 : x1) : s_prefix[v]; };
     const uint32_t ring = smem_u32(smem);
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp > kTokWarps) return;
         int v = v_first, issued = 0;
-        Group g = group_of(p.geo, p.rpg, v);
+        Group g = own;
         bool ok = true;
         // a block's page ids are fetched one block ahead (lane i: page i of the block)
         auto fetch = [&](int x, int &vv, Group &gg) {
@@ -347,13 +352,12 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             if (lane < p.pps && vp < gg.nv) {
                 const int pg = page_of(gg, vp);
                 if (pg < p.max_blocks) blk = p.block_table[(size_t)vv * p.max_blocks + pg];
-                if (blk < 0 || blk >= p.num_blocks) blk = -1;
             }
-            return blk;
+            return blk;  // as it comes: a look at it here would wait for the load
         };
-        int next = fetch(x0, v, g);
+        int next = p.whole && p.geo.window == 0 ? (lane < g.nv ? early : -1) : fetch(x0, v, g);
         for (int x = x0; x < x1; ++x, ++issued) {
-            const int blk = next;
+            const int blk = (uint32_t)next < (uint32_t)p.num_blocks ? next : -1;
             next = fetch(x + 1, v, g);
             const int st = issued % p.stages;
             if (issued >= p.stages)
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     int segs = 0;
     for (int x = x0; x < x1 && ok; ++segs) {
         while (x >= start(v + 1)) ++v;
-        const Group g = group_of(p.geo, p.rpg, v);
+        const Group g = v == v_first ? own : group_of(p.geo, p.rpg, v);
         const int seg1 = min(x1, start(v + 1));
         const bool whole = x == start(v) && seg1 == start(v + 1);
         const int slot = x == x0 ? 0 : 1;
@@ -658,13 +662,15 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         }
         if (p.kw > 1) {
             // The kw warps of each (head, tile) hold different pages' shares.  They leave them in
-            // shared memory (the last stage's, which has room for one row tile; with more tiles in
-            // a buffer behind the ring) and each finishes every kw-th row.  16-byte chunk 8 c + i of
+            // shared memory (the last stage's, which has room for one row tile and is free once all
+            // have read it; with more tiles, or a single segment and so no need of a long ring, in a
+            // buffer behind the ring) and each finishes every kw-th row.  16-byte chunk 8 c + i of
             // a row lies at 8 c + (i ^ (c | (row & 1) << 2)): free of bank conflicts both ways.
             const int st = (done - 1) % p.stages;
-            float *buf = reinterpret_cast<float *>(smem + (size_t)(p.ch == 1 ? st : p.stages) * stage_bytes) +
+            const bool own_buf = p.ch > 1 || p.whole;
+            float *buf = reinterpret_cast<float *>(smem + (size_t)(own_buf ? p.stages : st) * stage_bytes) +
                          (size_t)(h_of * p.ch + c_of) * p.kw * 16 * kHD;
-            ok = meet();  // every warp has read the stage
+            if (!own_buf) ok = meet();  // every warp has read the stage
             if (!ok) break;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -704,7 +710,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                         if (lane == 0) rec[kHD] = M, rec[kHD + 1] = L;
                     }
                 }
-            if (p.ch > 1) ok = meet();  // before the buffer's next use
+            if (p.ch > 1 && !p.whole) ok = meet();  // before the buffer's next use
             // reads and writes here come before the copies into this stage
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -1482,7 +1488,7 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
     const long long share = (blocks + t.G - 1) / t.G;
     // Or a CTA for each sequence and as few heads as the SMs allow: no partials, no second launch, whose
     // time is that of about four blocks (measured: 3 us, 0.8 us a block; one row over 301 keys 14.2 us
-    // with shares, 9.1 whole; 8 sequences in a 100-key window 18.7 and 7.7).
+    // with shares, 8.2 whole; 8 sequences in a 100-key window 18.7 and 7.0).
     for (int heads = 1; heads <= kTokWarps / t.ch; heads *= 2) {
         if (groups * ((nkv + heads - 1) / heads) > sms) continue;
         const TokPlan shares = t;
@@ -1496,7 +1502,7 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
         break;
     }
     t.stage_bytes = (size_t)t.pps * t.hg * 4096;
-    const size_t join = t.kw > 1 && t.ch > 1 ? (size_t)t.hg * t.ch * t.kw * 16 * kHD * sizeof(float) : 0;
+    const size_t join = t.kw > 1 && (t.ch > 1 || t.whole) ? (size_t)t.hg * t.ch * t.kw * 16 * kHD * sizeof(float) : 0;
     t.stages = (int)((kTokSmem - join) / t.stage_bytes);
     if (t.stages > kTokStages) t.stages = kTokStages;
     t.smem = t.stages * t.stage_bytes + join + 1024;
