@@ -217,8 +217,8 @@ __device__ __forceinline__ int cta_of(int x, int T, int G) {
 // The tcgen05 pipe does not fit these shapes: one token's rows (gsz = 4, say) would fill 4 of its
 // 128 rows.  mma.sync at 16 rows keeps up with HBM.
 //
-// Measured, in a captured graph: 96 verify rows over 32 x 8236 keys, 32 + 8 heads: 93.0 us with the
-// merge, 5.15 TB/s of cache, where the copy of as many bytes takes 74 us and this kernel with its
+// Measured, in a captured graph: 96 verify rows over 32 x 8236 keys, 32 + 8 heads: 93.5 us with the
+// merge, 5.1 TB/s of cache, where the copy of as many bytes takes 74 us and this kernel with its
 // arithmetic left out 89 (sums of pages differ by up to a block of 0.8 us between the CTAs, and the
 // first bytes arrive 5 us after the start).  One row over 131071 keys 54.8 us, 4.9 TB/s; one row over 301
 // keys 8.2 us, a chain of loads (lengths and page ids -> pages), two rounds of products and a join.
