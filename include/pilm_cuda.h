@@ -518,7 +518,7 @@ int ekernel_qk_norm_rope_kv_append_kv8_splitk(const ekernel_paged_attn_desc_t *d
  *    row's own (exact for elements down to 2^-28 of the row's largest), keys exactly; probabilities
  *    are rounded to f16 for the product with V; the output is rounded once, after the gate.
  *  - workspace: at least ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks)
- *    bytes, 16-byte aligned, its contents undefined before and after.  The library allocates
+ *    bytes (never 0, for an empty batch neither; 0 means a refused descriptor), 16-byte aligned, its contents undefined before and after.  The library allocates
  *    none of its own, so calls that may overlap on the GPU (other streams, other graphs) need
  *    only workspaces of their own.
  *  - max_q_len and max_context must bound the batch's rows and contexts: they size the

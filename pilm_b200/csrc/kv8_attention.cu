@@ -1581,6 +1581,7 @@ extern "C" {
 size_t ekernel_paged_attention_kv8_workspace_bytes(const ekernel_paged_attn_desc_t *desc, size_t window,
                                                    size_t sinks) {
     if (kv8_check_desc(desc, "ekernel_paged_attention_kv8_workspace_bytes") != ECPU_OK) return 0;
+    if (desc->total_q == 0 || desc->num_seqs == 0) return 256;  // nothing to plan; 0 is a refusal
     ChunkPlan c;
     if (plan_chunks(desc, window, sinks, c)) return c.part_bytes + 256;
     const TokPlan t = plan_tokens(desc, window, sinks);
