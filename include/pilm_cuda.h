@@ -476,7 +476,7 @@ int ekernel_silu_mul_f32(const float *gate_up, size_t rows, size_t inter, float 
  * v_scale [num_blocks, n_kv] fp32; an element is code * scale.  Half the bytes of the bf16
  * cache plus 1/512, so attention over long contexts, which is bound by reading the cache,
  * takes about half the time.  Page ids, slots and block tables mean what they do for the
- * bf16 cache.  Both caches 16-byte aligned; scales finite and not negative. ---- */
+ * bf16 cache.  Both caches 16-byte aligned; scales finite, and 0 or at least 2^-126. ---- */
 
 /* ekernel_qk_norm_rope_kv_append into an 8-bit cache.  Computed in fp32 with one rounding per
  * output (q to bf16, K and V to e4m3).
@@ -515,8 +515,11 @@ int ekernel_qk_norm_rope_kv_append_kv8_splitk(const ekernel_paged_attn_desc_t *d
  *  - A block id outside [0, num_blocks) reads as a page of zeros.  Bytes past the context are
  *    read as nothing whatever they hold; NaN codes (0x7F, 0xFF) below it must not occur.
  *  - Scores, softmax and sums are fp32.  Queries enter the product in f16 at a power of two of their
- *    row's own (exact for elements down to 2^-28 of the row's largest), keys exactly; probabilities
- *    are rounded to f16 for the product with V; the output is rounded once, after the gate.
+ *    row's own (exact for elements down to 2^-28 of the row's largest), keys exactly.  A key's
+ *    probability times its page's V scale, p * vs, is rounded to f16 for the product with V: 11 bits
+ *    down to 2^-23 of the largest p * vs among the keys that the row sees, steps of 2^-33 of it below
+ *    (a page of zero codes counts by its scale like any other).  The output is rounded once, after
+ *    the gate.
  *  - workspace: at least ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks)
  *    bytes (never 0, for an empty batch neither; 0 means a refused descriptor), 16-byte aligned, its contents undefined before and after.  The library allocates
  *    none of its own, so calls that may overlap on the GPU (other streams, other graphs) need

@@ -4,7 +4,11 @@
 // position p sees keys <= p, or with a window the keys in (p - window, p] and the first sinks.
 // With k = ks * K8 and v = vs * V8 of a page, codes K8 and V8 being f16 values exactly:
 //   s = (q . K8) * (ks / sqrt(128))      the scale of a page multiplies 16 scores, not 2048 codes
-//   o = sum_pages (vs / vref) * (p . V8) * vref / sum p,   vref the largest vs so far
+//   o = 2^d / sum 2^(s - m) * sum_pages (2^(s - m + log2 vs - d) . V8)
+// in base 2.  Each row has two running references: m for its scores, m + d for s + log2 vs over the keys
+// that it sees.  What goes into the product with V is thus held relative to the row's own largest
+// p * vs, and no page that it does not see, or gives no weight, takes bits from the others.  Both are
+// whole numbers, so with power-of-two scales every exponent here is formed without rounding.
 //
 // The reference's attention is FullAttention.forward (src/models/qwen3/attention.py:98-139);
 // it caches in the model's dtype, so there is no reference result to reproduce here: scores
@@ -92,18 +96,35 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float lg2(float x) {
+// log2 of a page's scale: exact for powers of two (lg2.approx is not), -inf for 0 and below 2^-126
+__device__ __forceinline__ float log2_scale(float x) {
+    const uint32_t b = __float_as_uint(x);
+    float e = (float)((int)(b >> 23) - 127);
     float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__uint_as_float((b & 0x7fffffu) | 0x3f800000u)));
+    e += b & 0x7fffffu ? y : 0.f;
+    return b < 0x800000u ? -INFINITY : e;
 }
 
 constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
-// Probabilities are held as 2^9 exp(s - m) in f16 for a reference m at most kLag below the running
-// maximum (in base 2): at most 2^15, with 11 bits down to 2^-23 of exp(m) and steps of 2^-33 below,
-// so a long tail of small ones still counts.  The lag spares most of the rescalings of O: a new
-// maximum within it leaves m where it is.
-constexpr float kProbBits = 9.f, kLag = 6.f;
+// The weights p * vs are held as 2^9 p vs / 2^M in f16 for a reference M = m + d at most kLag below
+// their running maximum (in base 2): below 2^16, with 11 bits down to 2^-23 of that maximum and
+// steps of 2^-33 below, so a long tail of small ones still counts.  The lag, which m has too, spares
+// most of the rescalings of O: a new maximum within it leaves the references where they are.
+constexpr float kProbBits = 9.f, kLag = 6.75f;
+// A page's log2 vs - d is held to this: below, its weights are nothing in f16, while its scores, which
+// come from the same exponentials, still count in the sum of p.
+constexpr float kLogFloor = -60.f;
+__device__ __forceinline__ float finite_or_0(float x) { return x == -INFINITY ? 0.f : x; }
+// O -> out: 2^d / l as two factors, neither of which leaves the normal range (g is 1 but near its ends)
+struct OutScale {
+    float f, g;
+};
+__device__ __forceinline__ OutScale out_scale(float d, float l) {
+    const bool lo = d < -100.f, hi = d > 100.f;
+    const float e = lo ? d + 64.f : (hi ? d - 64.f : d);
+    return {l > 0.f ? __fdiv_rn(ex2(e), l) : 0.f, lo ? 0x1p-64f : (hi ? 0x1p64f : 1.f)};
+}
 
 // x / (1 + exp(-gate)) of eight outputs
 __device__ __forceinline__ void apply_gate(float (&e)[8], const __nv_bfloat16 *gate) {
@@ -478,7 +499,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             plain1 = plain1 - g.lo_page + g.n_sink;
         }
 
-        float o[16][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f, inv_vref = 0.f;
+        float o[16][4], m[2] = {-INFINITY, -INFINITY}, d[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -501,12 +522,12 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                 const uint32_t vb = kb + p.pps * page_bytes;
                 const uint32_t valid = s_valid[st] >> (2 * k_of) & 3u;
                 const bool masked = vp < plain0 || vp + 2 > plain1 || valid != 3u;
-                float kf[2], vf[2];
+                float kf[2], lv[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int at = (2 * k_of + i) * p.hg + h_of;
                     kf[i] = s_scale[st][0][at];
-                    vf[i] = s_scale[st][1][at];
+                    lv[i] = log2_scale(s_scale[st][1][at]);
                 }
                 // ---- S = Q K8^T: two pages of two 8-key tiles, four independent chains ----
                 float s[2][2][4];
@@ -536,26 +557,16 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                 }
                 // ---- scores in base 2, masks, online softmax ----
                 // A page's K scale is a factor of its raw products, applied with the reference in one
-                // fma; its V scale is an addend there (p' = p * vs / vref), taken out of the sum again.
+                // fma; its V scale is an addend there (p' = p * vs / 2^d), taken out of the sum again.
                 float f[2][2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) f[i][0] = rowf[0] * kf[i], f[i][1] = rowf[1] * kf[i];
                 int key0[2] = {0, 0};
-                auto scale_scores = [&]() {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                        for (int t = 0; t < 2; ++t)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) s[i][t][j] *= f[i][j >> 1];
-                        f[i][0] = f[i][1] = 1.f;
-                    }
-                };
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const bool ok_page = (valid >> i) & 1u;
-                        if (!ok_page) vf[i] = 0.f;
+                        if (!ok_page) lv[i] = -INFINITY;
                         key0[i] = page_of(g, vp + i) * 16;
 #pragma unroll
                         for (int t = 0; t < 2; ++t)
@@ -570,45 +581,64 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                         f[i][0] = f[i][1] = 1.f;
                     }
                 }
-                float mx[2];
+                // this thread's largest score of each page, and whether any thread's moves a reference
+                float top[2][2];
+                bool rise = false, huge = false;
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
                     const int e = 2 * hh;
-                    mx[hh] = fmaxf(fmaxf(max3(s[0][0][e], s[0][0][e + 1], s[0][1][e]), s[0][1][e + 1]) * f[0][hh],
-                                   fmaxf(max3(s[1][0][e], s[1][0][e + 1], s[1][1][e]), s[1][1][e + 1]) * f[1][hh]);
-                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 1));
-                    mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(0xffffffffu, mx[hh], 2));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        top[i][hh] = fmaxf(max3(s[i][0][e], s[i][0][e + 1], s[i][1][e]), s[i][1][e + 1]) * f[i][hh];
+                    const float mx = fmaxf(top[0][hh], top[1][hh]), w = fmaxf(top[0][hh] + lv[0], top[1][hh] + lv[1]);
+                    rise |= mx > m[hh] + kLag || w > m[hh] + d[hh] + kLag;
+                    huge |= fabsf(mx) > 65536.f && mx > -INFINITY;
                 }
-                const float vtop = fmaxf(vref, fmaxf(vf[0], vf[1]));
-                // (the fma adds -m to an unrounded product, off by half a unit of m: scores past 2^16
-                // are rounded first, like m)
-                const bool huge = fabsf(mx[0]) > 65536.f || fabsf(mx[1]) > 65536.f;
-                if (__any_sync(0xffffffffu, mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || vtop > vref || huge)) {
-                    if (!masked && __any_sync(0xffffffffu, huge)) scale_scores();
-                    const float inv = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
-                    const float vfac = vref * inv;
-                    vref = vtop, inv_vref = inv;
+                // The exponents below add a page's log2 vs - d to -m, which past 2^16 would lose bits of
+                // it, and -m to an unrounded product: such scores are rounded and made relative to m first.
+                huge = __any_sync(0xffffffffu, huge);
+                if (huge || __any_sync(0xffffffffu, rise)) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
-                        const float mn = fmaxf(m[hh], mx[hh]);
-                        const float fm = mn == m[hh] ? 1.f : ex2(m[hh] - mn);  // first keys: ex2(-inf) = 0
-                        m[hh] = mn;
-                        l[hh] *= fm;
-                        const float fo = fm * vfac;
+                        float mx = fmaxf(top[0][hh], top[1][hh]), w = fmaxf(top[0][hh] + lv[0], top[1][hh] + lv[1]);
+#pragma unroll
+                        for (int x = 1; x <= 2; x *= 2) {
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, x));
+                        }
+                        const float mn = fmaxf(m[hh], floorf(mx)), mz = finite_or_0(mn);
+                        w -= mz;
+                        if (__builtin_expect(huge, 0)) {
+                            w = fmaxf((top[0][hh] - mz) + lv[0], (top[1][hh] - mz) + lv[1]);
+                            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 1));
+                            w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, 2));
+                        }
+                        const float dm = m[hh] - mz, dn = fmaxf(d[hh] + dm, floorf(w));  // first keys: dm = -inf
+                        const float fo = dn == -INFINITY ? 1.f : ex2(d[hh] + dm - dn);
+                        m[hh] = mn, d[hh] = dn;
+                        l[hh] *= ex2(dm);
 #pragma unroll
                         for (int n = 0; n < 16; ++n) o[n][2 * hh] *= fo, o[n][2 * hh + 1] *= fo;
+                        if (__builtin_expect(huge, 0))
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                                    for (int j = 2 * hh; j < 2 * hh + 2; ++j)
+                                        s[i][t][j] = __fmul_rn(s[i][t][j], f[i][hh]) - mz;
+                                f[i][hh] = 1.f;
+                            }
                     }
                 }
-                const float base[2] = {m[0] == -INFINITY ? 0.f : kProbBits - m[0],
-                                       m[1] == -INFINITY ? 0.f : kProbBits - m[1]};
                 uint32_t pa[2][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    // a page whose scale is 2^-60 of the largest or less counts for nothing in O
-                    const float lr = fmaxf(lg2(vf[i] * inv_vref), -60.f), back = ex2(-lr);
+                for (int hh = 0; hh < 2; ++hh) {
+                    const float base = huge ? kProbBits : kProbBits - finite_or_0(m[hh]), dz = finite_or_0(d[hh]);
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        const uint64_t ff = f2_pack(f[i][hh], f[i][hh]), cc = f2_pack(base[hh] + lr, base[hh] + lr);
+                    for (int i = 0; i < 2; ++i) {
+                        const float lr = fmaxf(lv[i] - dz, kLogFloor);
+                        const uint64_t ff = f2_pack(f[i][hh], f[i][hh]), cc = f2_pack(base + lr, base + lr);
                         float2 x[2];
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
@@ -616,7 +646,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                             x[t].x = ex2(x[t].x), x[t].y = ex2(x[t].y);
                             pa[i][2 * t + hh] = pack_f16(x[t].x, x[t].y);
                         }
-                        l[hh] = fmaf((x[0].x + x[0].y) + (x[1].x + x[1].y), back, l[hh]);
+                        l[hh] = fmaf((x[0].x + x[0].y) + (x[1].x + x[1].y), ex2(-lr), l[hh]);
                     }
                 }
                 // ---- O += P V8 ----
@@ -656,9 +686,12 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
             l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
             // O in its own units: a convex combination of the values
-            const float f = l[hh] > 0.f ? __fdiv_rn(vref, l[hh]) : 0.f;
+            const OutScale os = out_scale(d[hh], l[hh]);
 #pragma unroll
-            for (int n = 0; n < 16; ++n) o[n][2 * hh] *= f, o[n][2 * hh + 1] *= f;
+            for (int n = 0; n < 16; ++n) o[n][2 * hh] *= os.f, o[n][2 * hh + 1] *= os.f;
+            if (__any_sync(0xffffffffu, os.g != 1.f))
+#pragma unroll
+                for (int n = 0; n < 16; ++n) o[n][2 * hh] *= os.g, o[n][2 * hh + 1] *= os.g;
         }
         if (p.kw > 1) {
             // The kw warps of each (head, tile) hold different pages' shares.  They leave them in
@@ -871,7 +904,7 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
 // over S's 128), so S, P and O of both tiles fill the 512 TMEM columns, and while one tile's
 // softmax runs the tensor cores work on the other tile.  The softmax takes the row maximum page by
 // page on the raw products (a page's scale is one factor) and folds the page's V scale into the
-// exponent: p' = 2^(s f + c), c = bits - m + log2(vs / vref), one fma and one exp2 per score.
+// exponent: p' = 2^(s f + c), c = bits - m + log2 vs - d, one fma and one exp2 per score.
 // Register split of the 512 threads (128 each at launch, 65536): 176 for the softmax warps, 120 for
 // the converters, 40 for the issuer's group: 256 * 176 + 128 * 120 + 128 * 40 = 65536.  (With fewer the
 // converters spill, and a spilled load in flight waits for itself.)
@@ -992,7 +1025,7 @@ struct __align__(8) ChunkBars {
 __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ ChunkBars bar;
-    __shared__ __align__(16) float s_scale[kChScales][2][8];  // [block][K, V][page]
+    __shared__ __align__(16) float s_scale[kChScales][2][8];  // [block][K scale, log2 of the V scale][page]
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -1173,7 +1206,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
         for (int j = j0, n = 0; j < j1 && ok; ++j, ++n) {
             const int st = n & 1;
             const uint32_t parity = (uint32_t)((n >> 1) - 1) & 1u;
-            // scales of the block's pages (warp 8: lanes 0..7 K, 8..15 V); zero without a valid id
+            // scales of the block's pages (warp 8: lanes 0..7 K, 8..15 log2 of V); zero without a valid id
             float sc = 0.f;
             const bool cut = key_of(j * kChPages + lane) + kKv8Page > ctx;  // the context ends in the page
             uint32_t live = __ballot_sync(0xffffffffu, ids >= 0 && !cut);
@@ -1183,6 +1216,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                 const int blk = __shfl_sync(0xffffffffu, ids, lane & 7);
                 sc = (lane < 8 ? p.ks : p.vs)[(size_t)max(blk, 0) * p.nkv + kvh];
                 if (blk < 0) sc = 0.f;
+                if (lane >= 8) sc = log2_scale(sc);
             }
             const int next = fetch_ids(j + 1);
             if (n >= 2) ok = wait(&bar.k_empty[st], parity);
@@ -1239,7 +1273,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.q_full);
         }
-        float m = -INFINITY, l = 0.f, vref = 0.f, inv_vref = 0.f;
+        float m = -INFINITY, d = -INFINITY, l = 0.f;
         bool ok = true;
         if (t < tiles) {
             // positions of the warp's rows: pages [plain0, plain1) of the list, which all of them see
@@ -1256,11 +1290,11 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                 ok = wait(&bar.s_full[t], (uint32_t)n & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                float f[8], c2[8], vtop = vref;
+                float f[8], lv[8];
                 {
                     const float *sc = &s_scale[n % kChScales][0][0];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], c2[i] = sc[8 + i], vtop = fmaxf(vtop, c2[i]);
+                    for (int i = 0; i < 8; ++i) f[i] = rowf * sc[i], lv[i] = sc[8 + i];
                 }
                 const bool plain = j * kChPages >= plain0 && (j + 1) * kChPages <= plain1;
                 if (!plain) {
@@ -1284,7 +1318,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
 #pragma unroll
                     for (int i = 0; i < 8; ++i) f[i] = fmaxf(f[i], 1.17549435e-38f);
                 }
-                float mx = -INFINITY;  // page by page on the raw products
+                float mx = -INFINITY, top = -INFINITY;  // of s and s + log2 vs, page by page on the raw products
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t s[64];
@@ -1292,33 +1326,40 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                     tc_ld32(s_at + 64 * c + 32, s + 32);
                     tc_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, max16(s + 16 * i) * f[4 * c + i]);
-                }
-                // The fma below adds -m to an unrounded product: off by half a unit of m, which
-                // must stay far below 1.  Scores past 2^16 are rounded first, like m.
-                if (__any_sync(0xffffffffu, fabsf(mx) > 65536.f && mx > -INFINITY)) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t s[32];
-                        tc_ld32(s_at + 32 * c, s);
-                        tc_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * f[2 * c + (i >> 4)]);
-                        tc_st32(s_at + 32 * c, s);
+                    for (int i = 0; i < 4; ++i) {
+                        const float a = max16(s + 16 * i) * f[4 * c + i];
+                        mx = fmaxf(mx, a), top = fmaxf(top, a + lv[4 * c + i]);
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = 1.f;
-                    tc_st_wait();
                 }
-                if (__any_sync(0xffffffffu, mx > m + kLag || vtop > vref)) {
+                // The exponents below add a page's log2 vs - d to -m, which past 2^16 would lose bits of
+                // it, and -m to an unrounded product: such scores are rounded and made relative to m first.
+                const bool huge = __any_sync(0xffffffffu, fabsf(mx) > 65536.f && mx > -INFINITY);
+                if (huge || __any_sync(0xffffffffu, mx > m + kLag || top > m + d + kLag)) {
+                    const float mn = fmaxf(m, floorf(mx)), mz = finite_or_0(mn);
+                    float w = top - mz;
+                    if (huge) {
+                        w = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t s[32];
+                            tc_ld32(s_at + 32 * c, s);
+                            tc_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                s[i] = __float_as_uint(__fmul_rn(__uint_as_float(s[i]), f[2 * c + (i >> 4)]) - mz);
+                            w = max3(w, max16(s) + lv[2 * c], max16(s + 16) + lv[2 * c + 1]);
+                            tc_st32(s_at + 32 * c, s);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[i] = 1.f;
+                        tc_st_wait();
+                    }
                     // s_full of this block came after the products of the last one: O is complete
-                    const float inv = vtop >= 1.17549435e-38f ? __fdiv_rn(1.f, vtop) : 0.f;
-                    const float vfac = vref * inv, mn = fmaxf(m, mx);
-                    const float fm = mn == m ? 1.f : ex2(m - mn);
-                    vref = vtop, inv_vref = inv, m = mn;
-                    l *= fm;
+                    const float dm = m - mz, dn = fmaxf(d + dm, floorf(w));  // first keys: dm = -inf
+                    const float fo = dn == -INFINITY ? 1.f : ex2(d + dm - dn);
+                    m = mn, d = dn;
+                    l *= ex2(dm);
                     if (n > 0) {
-                        const float fo = fm * vfac;
 #pragma unroll 1
                         for (int c = 0; c < 8; ++c) {
                             uint32_t u[16];
@@ -1330,7 +1371,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : kProbBits - m;
+                const float base = huge ? kProbBits : kProbBits - finite_or_0(m), dz = finite_or_0(d);
                 // P over S, 32 scores at a time (their 16 columns of P lie over columns read before):
                 // two scores per fma, the sum of a page's with its V scale taken out again
 #pragma unroll
@@ -1340,7 +1381,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                     tc_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float lr = fmaxf(lg2(c2[2 * c + i] * inv_vref), -60.f);
+                        const float lr = fmaxf(lv[2 * c + i] - dz, kLogFloor);
                         const uint64_t ff = f2_pack(f[2 * c + i], f[2 * c + i]), cc = f2_pack(base + lr, base + lr);
                         uint64_t sum = 0ull;
 #pragma unroll
@@ -1366,7 +1407,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             if (ok && j0 < j1) ok = wait(&bar.o_done[t], 0);
             if (ok) {
                 tc_fence_after();
-                const float f = l > 0.f ? __fdiv_rn(vref, l) : 0.f;
+                const OutScale os = out_scale(d, l);
                 const size_t ob = qrow * kHD;
                 float *rec = p.splits > 1 ? p.part + ((size_t)split * p.total_q * p.nh + qrow) * kRec : nullptr;
 #pragma unroll 1
@@ -1379,7 +1420,10 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
                     }
                     if (!in) continue;
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) u[k] = j0 < j1 ? __float_as_uint(__uint_as_float(u[k]) * f) : 0u;
+                    for (int k = 0; k < 32; ++k) u[k] = j0 < j1 ? __float_as_uint(__uint_as_float(u[k]) * os.f) : 0u;
+                    if (os.g != 1.f)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * os.g);
                     if (rec) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
