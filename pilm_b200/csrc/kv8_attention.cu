@@ -125,6 +125,30 @@ __device__ __forceinline__ OutScale out_scale(float d, float l) {
     const float e = lo ? d + 64.f : (hi ? d - 64.f : d);
     return {l > 0.f ? __fdiv_rn(ex2(e), l) : 0.f, lo ? 0x1p-64f : (hi ? 0x1p64f : 1.f)};
 }
+// Partials of a row (reference m, sum l, output o of four dims) join by their shares of the sum so far, so
+// that o stays a convex combination of the values, in their range; a NaN partial gives NaN.
+struct Joined {
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    // U more (-inf and 0 where there is none)
+    template <int U>
+    __device__ __forceinline__ void add(const float (&m2)[U], const float (&l2)[U], const float4 (&o2)[U]) {
+        float mx = m, w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, m2[u]);
+        const float mb = finite_or_0(mx), had = l * ex2(m - mb);
+        m = mx, l = had;
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = l2[u] * ex2(m2[u] - mb), l += w[u];
+        const float inv = l > 0.f ? __frcp_rn(l) : 0.f, keep = had * inv;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float x = w[u] * inv;
+            o[0] += x * o2[u].x, o[1] += x * o2[u].y, o[2] += x * o2[u].z, o[3] += x * o2[u].w;
+        }
+    }
+};
 
 // x / (1 + exp(-gate)) of eight outputs
 __device__ __forceinline__ void apply_gate(float (&e)[8], const __nv_bfloat16 *gate) {
@@ -145,14 +169,14 @@ __device__ __forceinline__ void store8(__nv_bfloat16 *out, const float (&e)[8]) 
     }
     *reinterpret_cast<uint4 *>(out) = make_uint4(r[0], r[1], r[2], r[3]);
 }
-// four merged outputs o * f at element `at`
-__device__ __forceinline__ void finish4(__nv_bfloat16 *out, const __nv_bfloat16 *gate, size_t at, const float (&o)[4], float f) {
+// four merged outputs at element `at`
+__device__ __forceinline__ void finish4(__nv_bfloat16 *out, const __nv_bfloat16 *gate, size_t at, const float (&o)[4]) {
     uint2 gw = make_uint2(0u, 0u);
     if (gate) gw = *reinterpret_cast<const uint2 *>(gate + at);
     float e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        e[i] = o[i] * f;
+        e[i] = o[i];
         if (gate) {
             const uint32_t w = i < 2 ? gw.x : gw.y;
             const float gt = __uint_as_float((i & 1) ? (w & 0xffff0000u) : (w << 16));
@@ -721,26 +745,28 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             if (!ok) break;
             if (active)
                 for (int r = k_of; r < tile1 - tile0; r += p.kw) {
-                    const float2 *ml = &s_ml[segs & 1][warp - k_of][r];
-                    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
-                    for (int k = 0; k < p.kw; ++k) M = fmaxf(M, ml[16 * k].x);
-                    const float Mb = M == -INFINITY ? 0.f : M;
-                    for (int k = 0; k < p.kw; ++k) {
-                        const float w = ml[16 * k].y * ex2(ml[16 * k].x - Mb);
-                        const float4 v = *reinterpret_cast<const float4 *>(
-                            buf + (k * 16 + r) * kHD + 4 * ((lane & 24) + ((lane & 7) ^ (lane >> 3 | (r & 1) << 2))));
-                        L += w;
-                        O[0] += w * v.x, O[1] += w * v.y, O[2] += w * v.z, O[3] += w * v.w;
+                    Joined sum;
+                    float m2[kTokWarps], l2[kTokWarps];
+                    float4 o2[kTokWarps];
+#pragma unroll
+                    for (int k = 0; k < kTokWarps; ++k) {
+                        m2[k] = -INFINITY, l2[k] = 0.f, o2[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (k < p.kw) {
+                            const float2 ml = s_ml[segs & 1][warp - k_of + k][r];
+                            m2[k] = ml.x, l2[k] = ml.y;
+                            o2[k] = *reinterpret_cast<const float4 *>(
+                                buf + (k * 16 + r) * kHD + 4 * ((lane & 24) + ((lane & 7) ^ (lane >> 3 | (r & 1) << 2))));
+                        }
                     }
-                    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
+                    sum.add(m2, l2, o2);
                     const int rho = tile0 + r;
                     if (whole) {
-                        finish4(p.out, p.gate, ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD + 4 * lane, O, f);
+                        finish4(p.out, p.gate, ((size_t)(g.q0 + rho / p.geo.gsz) * p.nh + head * p.geo.gsz + rho % p.geo.gsz) * kHD + 4 * lane, sum.o);
                     } else {
                         float *rec = p.part + ((((size_t)blockIdx.y * p.G + cta) * 2 + slot) * p.hg * p.rpg +
                                                (size_t)h_of * p.rpg + rho) * kRec;
-                        *reinterpret_cast<float4 *>(rec + 4 * lane) = make_float4(O[0] * f, O[1] * f, O[2] * f, O[3] * f);
-                        if (lane == 0) rec[kHD] = M, rec[kHD + 1] = L;
+                        *reinterpret_cast<float4 *>(rec + 4 * lane) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+                        if (lane == 0) rec[kHD] = sum.m, rec[kHD + 1] = sum.l;
                     }
                 }
             if (p.ch > 1 && !p.whole) ok = meet();  // before the buffer's next use
@@ -791,7 +817,8 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
 // out before the wait for it, and one round of loads remains.
 template <int WPB, int U>
 __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, int wpi) {
-    __shared__ float s_o[WPB][kHD], s_ml[WPB][2];
+    __shared__ __align__(16) float s_o[WPB][kHD];
+    __shared__ float s_ml[WPB][2];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % wpi;
     const int per = WPB / wpi, hb = (p.nh + per - 1) / per;
@@ -822,7 +849,7 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
     const size_t rows = (size_t)p.hg * p.rpg;
     const float *base = p.part + ((size_t)(kvh / p.hg) * p.G * 2) * rows * kRec +
                         ((size_t)(kvh % p.hg) * p.rpg + rho) * kRec;
-    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
+    Joined sum;
     if (cut)
         for (int cb = c0 + sub * U; cb <= c1; cb += wpi * U) {
             float m[U], l[U];
@@ -849,45 +876,28 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
                 m[u] = none ? -INFINITY : ml[u].x, l[u] = none ? 0.f : ml[u].y;
                 if (none) o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            float mc = M;
-#pragma unroll
-            for (int u = 0; u < U; ++u) mc = fmaxf(mc, m[u]);
-            if (mc == -INFINITY) continue;
-            const float f = ex2(M - mc);
-            L *= f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[e] *= f;
-            M = mc;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float w = l[u] * ex2(m[u] - M);
-                L += w;
-                O[0] += w * o[u].x, O[1] += w * o[u].y, O[2] += w * o[u].z, O[3] += w * o[u].w;
-            }
+            sum.add(m, l, o);
         }
     if (wpi > 1) {
-        *reinterpret_cast<float4 *>(&s_o[warp][4 * lane]) = make_float4(O[0], O[1], O[2], O[3]);
-        if (lane == 0) s_ml[warp][0] = M, s_ml[warp][1] = L;
+        *reinterpret_cast<float4 *>(&s_o[warp][4 * lane]) = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+        if (lane == 0) s_ml[warp][0] = sum.m, s_ml[warp][1] = sum.l;
         __syncthreads();
         if (sub) return;
-        float mc = M;
-        for (int w = 1; w < wpi; ++w) mc = fmaxf(mc, s_ml[warp + w][0]);
-        const float mb = mc == -INFINITY ? 0.f : mc;
-        const float f = ex2(M - mb);
-        L *= f;
+        for (int w = 1; w < wpi; w += 4) {  // wpi is a power of two
+            float m[4], l[4];
+            float4 o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] *= f;
-        for (int w = 1; w < wpi; ++w) {
-            const float g = ex2(s_ml[warp + w][0] - mb);
-            L += s_ml[warp + w][1] * g;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[e] += g * s_o[warp + w][4 * lane + e];
+            for (int u = 0; u < 4; ++u) {
+                const int at = warp + min(w + u, wpi - 1);
+                m[u] = w + u < wpi ? s_ml[at][0] : -INFINITY, l[u] = w + u < wpi ? s_ml[at][1] : 0.f;
+                o[u] = *reinterpret_cast<const float4 *>(&s_o[at][4 * lane]);
+            }
+            sum.add(m, l, o);
         }
     }
     if (!cut) return;
     const size_t ob = ((size_t)(q0 + j) * p.nh + head) * kHD + 4 * lane;
-    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
-    finish4(p.out, p.gate, ob, O, f);
+    finish4(p.out, p.gate, ob, sum.o);
 }
 
 // ---------------------------------------------------------------------------------
@@ -1466,33 +1476,35 @@ __global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int nu
     const long long item = (long long)blockIdx.x * (8 / WPI) + warp / WPI;
     // rows of the batch only: those behind the last sequence are not written
     const bool in = item < (long long)p.geo.cu_q[num_seqs] * p.nh && item >= (long long)p.geo.cu_q[0] * p.nh;
-    float M = -INFINITY, L = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](float m, float l, const float4 &o) {
-        const float mn = fmaxf(M, m), mb = mn == -INFINITY ? 0.f : mn;
-        const float f = ex2(M - mb), w = l * ex2(m - mb);
-        M = mn, L = L * f + w;
-        O[0] = O[0] * f + w * o.x, O[1] = O[1] * f + w * o.y, O[2] = O[2] * f + w * o.z, O[3] = O[3] * f + w * o.w;
-    };
-    if (in) {
-#pragma unroll 4
-        for (int s = part; s < p.splits; s += WPI) {
-            const float *rec = p.part + ((size_t)s * p.total_q * p.nh + item) * kRec;
-            add(rec[kHD], rec[kHD + 1], *reinterpret_cast<const float4 *>(rec + 4 * lane));
+    Joined sum;
+    float m[4], l[4];
+    float4 o[4];
+    if (in)
+        for (int s = part; s < p.splits; s += 4 * WPI) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const bool is = s + u * WPI < p.splits;
+                const float *rec = p.part + ((size_t)(is ? s + u * WPI : part) * p.total_q * p.nh + item) * kRec;
+                const float2 ml = *reinterpret_cast<const float2 *>(rec + kHD);
+                m[u] = is ? ml.x : -INFINITY, l[u] = is ? ml.y : 0.f;
+                o[u] = is ? *reinterpret_cast<const float4 *>(rec + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            sum.add(m, l, o);
         }
-    }
     if (WPI > 1) {
-        // a partial sum as a record: O / L with weight L
-        const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
-        s_o[warp][lane] = make_float4(O[0] * f, O[1] * f, O[2] * f, O[3] * f);
-        if (lane == 0) s_ml[warp] = make_float2(M, L);
+        s_o[warp][lane] = make_float4(sum.o[0], sum.o[1], sum.o[2], sum.o[3]);
+        if (lane == 0) s_ml[warp] = make_float2(sum.m, sum.l);
         __syncthreads();
         if (part) return;
+        float m7[WPI], l7[WPI];  // the others' sums
+        float4 o7[WPI];
+        m7[0] = -INFINITY, l7[0] = 0.f, o7[0] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 1; i < WPI; ++i) add(s_ml[warp + i].x, s_ml[warp + i].y, s_o[warp + i][lane]);
+        for (int i = 1; i < WPI; ++i) m7[i] = s_ml[warp + i].x, l7[i] = s_ml[warp + i].y, o7[i] = s_o[warp + i][lane];
+        sum.add(m7, l7, o7);
     }
     if (!in) return;
-    const float f = L > 0.f ? __fdiv_rn(1.f, L) : 0.f;
-    finish4(p.out, p.gate, (size_t)item * kHD + 4 * lane, O, f);
+    finish4(p.out, p.gate, (size_t)item * kHD + 4 * lane, sum.o);
 }
 
 // ---------------------------------------------------------------------------------

@@ -136,7 +136,7 @@ def test_scales_of_zero(q_lens, ctxs, nh, nkv):
 
 
 @pytest.mark.parametrize("q_lens,ctxs,nh,nkv", SHAPES)
-@pytest.mark.parametrize("e", [-126, -110, 90])
+@pytest.mark.parametrize("e", [-126, -110, 90, 110, 118])
 def test_ends_of_the_scales_range(q_lens, ctxs, nh, nkv, e):
     run(q_lens, ctxs, nh, nkv, lambda i, n: e, seed=7)
     run(q_lens, ctxs, nh, nkv, lambda i, n: e if i % 2 else (-126 if e > 0 else -100), seed=8)
@@ -160,3 +160,34 @@ def test_scales_that_are_no_powers_of_two(q_lens, ctxs, nh, nkv):
                 vs[page] *= 1.0 + 0.37 * ((5 * i + 3 * j) % 7) / 7
                 ks[page] *= 1.0 + 0.41 * ((3 * i + 5 * j) % 5) / 5
     run(q_lens, ctxs, nh, nkv, lambda i, n: -7 + 9 * (i % 3), seed=10, edit=edit)
+
+
+@pytest.mark.parametrize("q_lens,ctxs,nh,nkv", SHAPES + [([2], [9000], 32, 8), ([1] * 3, [4000, 3000, 5000], 64, 4),
+                                                         ([12], [9000], 32, 8)])
+def test_a_nan_query_gives_nan(q_lens, ctxs, nh, nkv):
+    """Also where its row is put together from partials."""
+    d = dev()
+    b = ref.batch(q_lens, ctxs, 11)
+    q = torch.randn((b.total, nh * HD), generator=torch.Generator(device=d).manual_seed(11), device=d).to(torch.bfloat16)
+    q[0, HD + 5] = math.nan
+    out = torch.empty_like(q)
+    ck.paged_attention_verify_kv8(make_desc(b, nh, nkv), q, *ref.random_cache(b.blocks, nkv, 12, d), table_of(b),
+                                  i32(b.cu), i32(ctxs), None, out)
+    bad = out.isnan().view(b.total, nh, HD)
+    assert bad[0, 1].all() and int(bad.sum()) == HD
+
+
+@pytest.mark.parametrize("tail", [0, 3000])
+def test_more_splits_than_lanes(tail):
+    """One sequence of 40 rows over many keys takes 64 splits, with rows behind it that are not its own."""
+    d, nh, nkv = dev(), 4, 1
+    b = ref.batch([10], [5000], 13)
+    g = torch.Generator(device=d).manual_seed(13)
+    q = (torch.randn((b.total + tail, nh * HD), generator=g, device=d) * 1.5).to(torch.bfloat16)
+    cache = ref.random_cache(b.blocks, nkv, 14, d)
+    desc = make_desc(b, nh, nkv, max_ctx=5000 * 16)  # a bound: more blocks are planned than there are
+    desc.total_q = b.total + tail
+    out = torch.full(q.shape, 7.25, dtype=torch.bfloat16, device=d)
+    ck.paged_attention_verify_kv8(desc, q, *cache, table_of(b), i32(b.cu), i32(b.ctxs), None, out)
+    assert (out[b.total:] == 7.25).all()
+    check(out[:b.total], restated(q[:b.total], *cache, b, nkv, 0, 0), 5000)
