@@ -96,14 +96,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// log2 of a page's scale: exact for powers of two (lg2.approx is not), -inf for 0 and below 2^-126
+// log2 of a page's scale, -inf for 0 and below 2^-126.  Exact for powers of two, which lg2.approx below 1
+// is not: the exponent (as a float: 2^23 + its bits) plus the logarithm of the significand, 0 at 1.
 __device__ __forceinline__ float log2_scale(float x) {
     const uint32_t b = __float_as_uint(x);
-    float e = (float)((int)(b >> 23) - 127);
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__uint_as_float((b & 0x7fffffu) | 0x3f800000u)));
-    e += b & 0x7fffffu ? y : 0.f;
-    return b < 0x800000u ? -INFINITY : e;
+    y += __uint_as_float((b >> 23) | 0x4b000000u) - 8388735.f;
+    return b < 0x800000u ? -INFINITY : y;
 }
 
 constexpr float kScoreScale = 0.08838834764831845f * 1.4426950408889634f;  // log2(e) / sqrt(128)
@@ -524,6 +524,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         }
 
         float o[16][4], m[2] = {-INFINITY, -INFINITY}, d[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float base[2] = {kProbBits, kProbBits}, dz[2] = {0.f, 0.f};  // kProbBits - m and d, with 0 for -inf
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -640,6 +641,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                         const float dm = m[hh] - mz, dn = fmaxf(d[hh] + dm, floorf(w));  // first keys: dm = -inf
                         const float fo = dn == -INFINITY ? 1.f : ex2(d[hh] + dm - dn);
                         m[hh] = mn, d[hh] = dn;
+                        base[hh] = kProbBits - mz, dz[hh] = finite_or_0(dn);
                         l[hh] *= ex2(dm);
 #pragma unroll
                         for (int n = 0; n < 16; ++n) o[n][2 * hh] *= fo, o[n][2 * hh + 1] *= fo;
@@ -658,11 +660,11 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
                 uint32_t pa[2][4];
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    const float base = huge ? kProbBits : kProbBits - finite_or_0(m[hh]), dz = finite_or_0(d[hh]);
+                    const float at = huge ? kProbBits : base[hh];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float lr = fmaxf(lv[i] - dz, kLogFloor);
-                        const uint64_t ff = f2_pack(f[i][hh], f[i][hh]), cc = f2_pack(base + lr, base + lr);
+                        const float lr = fmaxf(lv[i] - dz[hh], kLogFloor);
+                        const uint64_t ff = f2_pack(f[i][hh], f[i][hh]), cc = f2_pack(at + lr, at + lr);
                         float2 x[2];
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
