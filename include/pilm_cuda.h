@@ -480,8 +480,8 @@ int ekernel_silu_mul_f32(const float *gate_up, size_t rows, size_t inter, float 
 
 /* ekernel_qk_norm_rope_kv_append into an 8-bit cache.  Computed in fp32 with one rounding per
  * output (q to bf16, K and V to e4m3).
- *  - A page's new scale is 2^e, e the least integer with amax <= 448 * 2^e, amax being the
- *    largest magnitude among the rows written now and the tokens kept (0 gives e = 0).  Kept
+ *  - A page's new scale is 2^e, e the least integer from -126 on with amax <= 448 * 2^e, amax being
+ *    the largest magnitude among the rows written now and the tokens kept (0 gives e = 0).  Kept
  *    are the tokens at offsets below the first offset written: their codes are rounded to the
  *    new scale.  Tokens above (rejected drafts, an earlier owner's) are stale and count for
  *    nothing, so a row at offset 0 starts its page anew.

@@ -5,7 +5,7 @@
 // into a page join the tokens at offsets below the first of them (the page's kept tokens; what
 // lies above is stale: rejected drafts, an earlier owner's tokens).  With
 //   amax = max |x| over the kept tokens (as stored) and the new rows,
-//   e    = the least integer with amax <= 448 * 2^e   (0 for an all-zero page)
+//   e    = the least integer from -126 on with amax <= 448 * 2^e   (0 for an all-zero page)
 // the page's scale becomes 2^e, the kept codes are rounded to it and the new rows stored as
 // rne_e4m3(x * 2^-e).  A power of two costs an e4m3 value nothing (its exponent moves), so
 // requantizing kept tokens is exact except where a code becomes subnormal, and a page holds
@@ -216,7 +216,7 @@ __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
     return r;
 }
 
-// The exponent e of a page's scale: the least with amax <= 448 * 2^e (448 = 1.75 * 2^8).
+// The exponent e of a page's scale: the least from -126 on with amax <= 448 * 2^e (448 = 1.75 * 2^8).
 __device__ __forceinline__ int scale_exponent(float amax) {
     if (!(amax > 0.f)) return 0;
     const uint32_t b = __float_as_uint(amax);
@@ -332,7 +332,9 @@ __device__ __forceinline__ void append_run(const AppendParams &p, int lead, int 
     amax = fmaxf(s_amax[warp & ~1], s_amax[warp | 1]);
     const int e = scale_exponent(amax);
     const float new_scale = pow2f(e), inv = pow2f(-e);
-    const bool rescale = lo > 0 && new_scale != old_scale;
+    // kept zeros stay as they are: the ratio of the scales may be infinite there (elsewhere it is at most
+    // 2^18: the largest kept value, at least 2^-9 * old_scale, is at most 448 * new_scale)
+    const bool rescale = kept_max > 0.f && new_scale != old_scale;
     const float f = old_scale * inv;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
