@@ -23,7 +23,9 @@ static __device__ int g_kv8_error;
 namespace {
 
 constexpr int kHD = kKv8HD;
-constexpr uint32_t kWaitLimit = 1u << 20;  // polls, of about two microseconds each, before a wait gives up
+// Polls, of about two microseconds each, before a wait gives up (ekernel_set_wait_limit's instead where
+// set; the waits for what is in flight at the end keep this one).
+constexpr uint32_t kWaitLimit = 1u << 20;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint64_t *b, uint32_t count) {
@@ -46,13 +48,30 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Bounded wait; false once the limit is reached or another warp gave up (unless abort_flag is null).
-__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag) {
-    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+__device__ __forceinline__ bool mbar_test(uint64_t *b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait; false once it has polled `limit` times (0: if it is not met now) or another warp gave up.
+__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, volatile int *abort_flag, uint32_t limit) {
+    if (mbar_test(b, parity)) return true;
+    for (uint32_t i = 0; i < limit; ++i) {
         if (mbar_try_wait(b, parity)) return true;
-        if (abort_flag && (i & 255) == 255 && *abort_flag) return false;
+        if ((i & 255) == 255 && *abort_flag) return false;
     }
     return false;
+}
+// A wait for what always completes, before the CTA may exit.
+__device__ __forceinline__ void mbar_drain(uint64_t *b, uint32_t parity) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i)
+        if (mbar_try_wait(b, parity)) return;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
     asm volatile(
@@ -289,6 +308,7 @@ struct TokParams {
     int nh, nkv, max_blocks, num_blocks;
     int groups, hg, ch, kw, pps, rpg, stages, G;  // groups: sequences; rpg = 16 ch rows of each
     int whole;  // a CTA per group (and head group) instead of equal shares of all pages
+    uint32_t wait_limit;
 };
 
 // Rows of a group that sees no key.
@@ -406,7 +426,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
             next = fetch(x + 1, v, g);
             const int st = issued % p.stages;
             if (issued >= p.stages)
-                ok = mbar_wait(&empty_bar[st], (uint32_t)(issued / p.stages - 1) & 1u, &s_abort);
+                ok = mbar_wait(&empty_bar[st], (uint32_t)(issued / p.stages - 1) & 1u, &s_abort, p.wait_limit);
             if (!__all_sync(0xffffffffu, ok)) break;
             const uint32_t valid = __ballot_sync(0xffffffffu, blk >= 0);
             if (lane == 0) {
@@ -435,7 +455,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
         }
         // every copy issued lands before the CTA may exit
         for (int j = issued > p.stages ? issued - p.stages : 0; j < issued; ++j)
-            mbar_wait(&full_bar[j % p.stages], (uint32_t)(j / p.stages) & 1u, nullptr);
+            mbar_drain(&full_bar[j % p.stages], (uint32_t)(j / p.stages) & 1u);
         return;
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -456,7 +476,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
     auto meet = [&]() {
         __syncwarp();
         if (lane == 0) mbar_arrive(&meet_bar);
-        const bool w = __all_sync(0xffffffffu, mbar_wait(&meet_bar, (uint32_t)met++ & 1u, &s_abort));
+        const bool w = __all_sync(0xffffffffu, mbar_wait(&meet_bar, (uint32_t)met++ & 1u, &s_abort, p.wait_limit));
         if (!w && lane == 0) {
             s_abort = 1;
             atomicExch(&g_kv8_error, 1);
@@ -532,7 +552,7 @@ __global__ void __launch_bounds__(kTokThreads, 1) kv8_attn_tokens(const __grid_c
 
         for (; x < seg1; ++x, ++done) {
             const int st = done % p.stages;
-            ok = mbar_wait(&full_bar[st], (uint32_t)(done / p.stages) & 1u, &s_abort);
+            ok = mbar_wait(&full_bar[st], (uint32_t)(done / p.stages) & 1u, &s_abort, p.wait_limit);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) {
                     s_abort = 1;
@@ -949,6 +969,7 @@ struct ChunkParams {
     __nv_bfloat16 *out;
     float *part;  // [splits][total_q][nh][kRec], when splits > 1
     int nh, nkv, max_blocks, num_blocks, total_q, rgs, splits;  // rgs: groups of kChRows rows per sequence
+    uint32_t wait_limit;
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -1033,7 +1054,7 @@ struct __align__(8) ChunkBars {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_done[2], drain;
 };
 
-// grid: (sequences x groups x splits, n_kv)
+// grid: groups of rows (the last first) x sequences x KV heads x splits
 __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ ChunkBars bar;
@@ -1095,7 +1116,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
     auto key_of = [&](int i) { return (i < n_sink ? i : i - n_sink + lo_page) * kKv8Page; };  // page i's first
     // a wait of the whole warp; false once any lane gave up
     auto wait = [&](uint64_t *m, uint32_t parity) {
-        const bool ok = __all_sync(0xffffffffu, mbar_wait(m, parity, &s_abort));
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(m, parity, &s_abort, p.wait_limit));
         if (!ok) *(volatile int *)&s_abort = 1;
         return ok;
     };
@@ -1160,7 +1181,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_attn_chunk(const ChunkParam
             // everything issued has completed (also when a wait gave up)
             if (lane == 0) tc_commit(&bar.drain);
             __syncwarp();
-            mbar_wait(&bar.drain, 0, nullptr);
+            mbar_drain(&bar.drain, 0);
             if (!ok && lane == 0) atomicExch(&g_kv8_error, 1);
             __syncwarp();
         }
@@ -1670,6 +1691,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
     geo.gsz = (int)(desc->n_heads / desc->n_kv_heads);
     geo.window = window >= cap ? 0 : (int)window;
     geo.sinks = (int)(sinks < cap ? sinks : cap);
+    const uint32_t limit = wait_limit_override() >= 0 ? (uint32_t)wait_limit_override() : kWaitLimit;
     ChunkPlan c;
     if (plan_chunks(desc, window, sinks, c)) {
         PILM_REQUIRE(c.ctas <= 0x7fffffffLL, ECPU_ERR_PARAM, "%s: too many rows", what);
@@ -1691,6 +1713,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.num_blocks = (int)desc->num_blocks;
         p.total_q = (int)desc->total_q;
         p.splits = c.splits;
+        p.wait_limit = limit;
         cudaFuncSetAttribute(kv8_attn_chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kChSmem);
         launch_pdl(kv8_attn_chunk, dim3((unsigned)c.ctas), dim3(kChThreads),
                    kChSmem, p);
@@ -1736,6 +1759,7 @@ int ekernel_paged_attention_verify_kv8(const ekernel_paged_attn_desc_t *desc, co
         p.stages = t.stages;
         p.G = t.G;
         p.whole = t.whole;
+        p.wait_limit = limit;
         launch_pdl(kv8_attn_tokens, dim3((unsigned)t.G, (unsigned)t.ngroups), dim3(kTokThreads), t.smem,
                    maps[0], maps[1], p);
         rc = check_launch(what);
