@@ -3,10 +3,12 @@
     python -m pilm_b200.build            # or: import pilm_b200.build; build()
 
 and _args.so, the Python entry of the 8-bit KV cache calls (csrc/args.cpp), with g++ against
-torch's headers.
+torch's headers.  The library comes first and needs nvcc alone; a host without torch, Python's
+headers or a C++ compiler gets it all the same, with a warning that _args.so was left out.
 
-The library is written next to this file so that it ships with the package and
-with snapshots of the repository; it is rebuilt only when a source is newer.
+Both are written next to this file so that they ship with the package and with snapshots of
+the repository; they are rebuilt only when a source is newer, _args.so also when it was built
+for another torch or Python.
 """
 from __future__ import annotations
 
@@ -14,12 +16,16 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
+from importlib import metadata, util
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 LIB = HERE / "libpilm_cuda.so"
 ARGS = HERE / "_args.so"
+ARGS_STAMP = HERE / "_build" / "args.stamp"  # what the built _args.so was built for
 INCLUDE = HERE.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["runtime.cu", "linear.cu", "linear_tc.cu", "norm.cu", "attention.cu", "accept.cu", "mtp.cu", "f32.cu",
@@ -41,29 +47,66 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > t for p in deps if p.exists())
 
 
+def cxx() -> str:
+    return os.environ.get("CXX") or "g++"
+
+
+def args_missing() -> str:
+    """What this host lacks of what _args.so is built from; empty when nothing."""
+    if util.find_spec("torch") is None:
+        return "torch is not installed"
+    header = Path(sysconfig.get_paths()["include"]) / "Python.h"
+    if not header.exists():
+        return f"{header} does not exist"
+    if not shutil.which(cxx().split()[0]):
+        return f"no C++ compiler ({cxx()})"
+    return ""
+
+
+def _args_target() -> str:
+    return f"torch {metadata.version('torch')} {sysconfig.get_config_var('SOABI')}"
+
+
 def build_args(force: bool = False) -> Path:
     """_args.so: a Python extension module on torch's C++ API."""
     src = CSRC / "args.cpp"
     deps = [src] + list(INCLUDE.glob("*.h"))
-    if not force and ARGS.exists() and all(p.stat().st_mtime <= ARGS.stat().st_mtime for p in deps):
+    target = _args_target()
+    if (not force and ARGS.exists() and all(p.stat().st_mtime <= ARGS.stat().st_mtime for p in deps)
+            and ARGS_STAMP.exists() and ARGS_STAMP.read_text() == target):
         return ARGS
-    import sysconfig
-
     import torch
     root = Path(torch.__file__).resolve().parent
     tmp = ARGS.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-           "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
-           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), str(src),
-           "-L", str(root / "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", str(tmp)]
-    subprocess.run(cmd, check=True)
+    cmd = cxx().split() + [
+        "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        "-I", sysconfig.get_paths()["include"], "-isystem", str(root / "include"),
+        "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"), str(src),
+        "-L", str(root / "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", str(tmp)]
+    try:
+        subprocess.run(cmd, check=True)
+    except subprocess.CalledProcessError as e:
+        raise RuntimeError(f"{ARGS.name}, the Python entry of the 8-bit KV cache calls, did not build ({LIB.name} did): "
+                           f"{' '.join(cmd)}") from e
     os.replace(tmp, ARGS)
+    ARGS_STAMP.parent.mkdir(exist_ok=True)
+    ARGS_STAMP.write_text(target)
     return ARGS
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    build_args(force)
+    build_library(force, verbose)
+    missing = args_missing()
+    if missing:
+        warnings.warn(f"{ARGS.name} was not built: {missing}. {LIB.name} is complete; the 8-bit KV cache calls of "
+                      "pilm_b200.ckernel need both")
+    else:
+        build_args(force)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return LIB
     objdir = HERE / "_build"
