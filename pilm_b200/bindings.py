@@ -256,9 +256,12 @@ def args():
     global _args
     if _args is None:
         try:
+            import torch  # noqa: F401  (loads the libraries that the extension is linked against)
+
             from . import _args as module
         except ImportError as e:
-            raise RuntimeError("pilm_b200/_args.so could not be loaded: build it with `python -m pilm_b200.build`") from e
+            raise RuntimeError("pilm_b200/_args.so could not be loaded (build it with `python -m pilm_b200.build`): "
+                               f"{e}") from e
         L = _load_lib()
         module.bind(*(ctypes.cast(getattr(L, n), _vp).value for n in
                       ("ekernel_qk_norm_rope_kv_append_kv8", "ekernel_qk_norm_rope_kv_append_kv8_splitk",

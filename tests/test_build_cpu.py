@@ -1,5 +1,6 @@
 """The build's order and conditions, with the compilers replaced by a recorder."""
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -73,3 +74,19 @@ def test_another_torch_rebuilds_the_extension_alone(tree, monkeypatch):
     assert runs == ["_args.so.tmp"]
     b.build()
     assert runs == ["_args.so.tmp"]
+
+
+def test_the_extension_loads_in_a_process_that_has_not_imported_torch():
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", "from pilm_b200 import bindings; print(bindings.args().__name__)"], cwd=root,
+                       capture_output=True, text=True, timeout=300)
+    assert r.stdout.strip() == "pilm_b200._args", r.stderr
+
+
+def test_an_extension_that_does_not_load_says_why(monkeypatch):
+    from pilm_b200 import bindings
+    monkeypatch.setattr(bindings, "_args", None)
+    monkeypatch.setitem(sys.modules, "pilm_b200._args", None)
+    monkeypatch.delattr(sys.modules["pilm_b200"], "_args", raising=False)
+    with pytest.raises(RuntimeError, match="python -m pilm_b200.build.*: .*_args"):
+        bindings.args()
