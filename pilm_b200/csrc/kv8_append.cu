@@ -456,8 +456,8 @@ int append(const ekernel_paged_attn_desc_t *d, const uint16_t *qkv, const float 
     PILM_REQUIRE(aligned(k_cache, 16) && aligned(v_cache, 16), ECPU_ERR_PARAM,
                  "%s: the K and V caches must be 16-byte aligned", what);
     const size_t width = (d->n_heads * (d->output_gate ? 2 : 1) + 2 * d->n_kv_heads) * kHD;
-    PILM_REQUIRE(d->qkv_stride >= width, ECPU_ERR_PARAM, "%s: qkv_stride %zu is below the row's %zu values", what,
-                 d->qkv_stride, width);
+    PILM_REQUIRE(d->qkv_stride >= width && d->qkv_stride <= 0x7fffffff, ECPU_ERR_PARAM,
+                 "%s: qkv_stride %zu is not in [%zu, 2^31), from the row's values on", what, d->qkv_stride, width);
     AppendParams p;
     p.qkv = (const __nv_bfloat16 *)qkv;
     p.part = part;
@@ -522,6 +522,7 @@ int kv8_check_desc(const ekernel_paged_attn_desc_t *d, const char *what) {
                  "%s: sizes out of range", what);
     PILM_REQUIRE(d->num_blocks > 0 && d->num_blocks < (1u << 27), ECPU_ERR_PARAM,
                  "%s: num_blocks must be in [1, 2^27)", what);
+    PILM_REQUIRE(d->max_blocks_per_seq <= 0x7fffffff, ECPU_ERR_PARAM, "%s: max_blocks_per_seq must be below 2^31", what);
     PILM_REQUIRE(d->rot_dim <= kKv8HD && (d->rot_dim & 1) == 0 && d->rope_rows <= 0x7fffffff, ECPU_ERR_PARAM,
                  "%s: bad rot_dim or rope_rows", what);
     return ECPU_OK;

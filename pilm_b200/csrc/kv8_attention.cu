@@ -1533,6 +1533,10 @@ __global__ void __launch_bounds__(256) kv8_attn_join(const ChunkParams p, int nu
 // ---------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------
+long long max_keys(const ekernel_paged_attn_desc_t *d) {  // a larger bound bounds no more: contexts are int32
+    return d->max_context < 0x7fffffff ? (long long)d->max_context : 0x7fffffff;
+}
+
 struct TokPlan {
     int hg, ngroups, ch, kw, pps, G, whole, stages;
     size_t stage_bytes, smem, part_bytes, prefix_bytes;
@@ -1545,7 +1549,7 @@ TokPlan plan_tokens(const ekernel_paged_attn_desc_t *d, size_t window, size_t si
     const int nkv = (int)d->n_kv_heads, gsz = (int)(d->n_heads / d->n_kv_heads), sms = num_sms();
     const long long max_q = (long long)(d->max_q_len < 1 ? 1 : (d->max_q_len < d->total_q ? d->max_q_len : d->total_q));
     t.ch = (int)(max_q * gsz + 15) / 16;  // 1 or 2 row tiles share the pages that a CTA reads
-    long long keys = (long long)d->max_context;
+    long long keys = max_keys(d);
     if (window > 0 && window < (1u << 30) && sinks < (1u << 30)) {
         const long long seen = (long long)window + (long long)sinks + max_q + 32;
         if (seen < keys) keys = seen;
@@ -1609,7 +1613,7 @@ bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks
     if (max_q * gsz < kChunkRows) return false;
     c.rgs = (int)((max_q * gsz + kChRows - 1) / kChRows);
     const long long ctas = (long long)d->num_seqs * c.rgs * (long long)d->n_kv_heads;
-    long long keys = (long long)d->max_context;
+    long long keys = max_keys(d);
     if (window > 0 && window < (1u << 30) && sinks < (1u << 30)) {
         const long long seen = (long long)window + (long long)sinks + max_q + 2 * kChKeys;
         if (seen < keys) keys = seen;
