@@ -84,6 +84,25 @@ def bench_config(layers: int, world: int, seqs: int = SEQS, prompt: int = PROMPT
     }
 
 
+def kv_config(args) -> dict:
+    """What a line says of a cache that is not the default workload's."""
+    return {"kv_cache": "e4m3", "window": args.window, "sinks": args.sinks} if args.kv == "e4m3" else {}
+
+
+def check_kv_flags(ap, args) -> None:
+    """--kv, --window and --sinks where a run would not use them end it, rather than being passed over."""
+    if args.window < 0 or args.sinks < 0:
+        ap.error("--window and --sinks must not be negative")
+    if args.kv != "e4m3" and (args.window or args.sinks):
+        ap.error("--window and --sinks need --kv e4m3")
+    if args.sinks and not args.window:
+        ap.error("--sinks needs --window")
+    other = [f for f, on in (("--sweep", args.sweep and not args.prefill), ("--config", args.config and not args.prefill),
+                             ("--impl reference", args.impl == "reference")) if on]
+    if args.kv != "bf16" and other:
+        ap.error(f"{other[0]} runs on its own cache: --kv {args.kv} is for the bench line and --prefill")
+
+
 def peaks() -> dict:
     p = ROOT / "MEASURED_PEAKS.json"
     if p.exists():
@@ -448,10 +467,11 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
         "higher_is_better": True,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "bf16 activations x int4 weights, fp32 accumulate",
+        "dtype": "bf16 activations x int4 weights, fp32 accumulate" + (", e4m3 KV cache" if kv8 else ""),
         "data": "synthetic (seeded random-init weights, random prompt KV pages, random drafts)",
-        "config": dict(bench_config(shape.layers, world, SEQS, PROMPT),
-                       **({"kv_cache": "e4m3", "window": args.window, "sinks": args.sinks} if kv8 else {})),
+        "config": dict(bench_config(shape.layers, world, SEQS, PROMPT), **kv_config(args),
+                       **({"l2": f"inputs larger than L2 (about {att_bytes * shape.layers / 1e9:.2g} GB KV + "
+                                 f"{lin_bytes / 1e9:.2g} GB weights read per step)"} if kv8 else {})),
         "per_gpu": round(value / world, 2),
         "e2e": {
             "value": round(e2e_rows_all / max(1, e2e_steps) / (e2e_ms_max * 1e-3), 2) if e2e_steps else None,
@@ -899,20 +919,22 @@ def run_prefill(args) -> None:
 
     from pilm_b200 import bindings
     from pilm_b200.engine import MTPVerifyEngine
-    from pilm_b200.qwen3 import QWEN3_8B, PagedKVCache, Qwen3Verifier, Qwen3Weights
+    from pilm_b200.qwen3 import QWEN3_8B, PagedKVCache, PagedKVCacheKV8, Qwen3Verifier, Qwen3Weights
 
     dev = torch.device("cuda", 0)
     torch.cuda.set_device(dev)
     bindings.init()
     shape = QWEN3_8B
     P = args.prefill
+    cache = PagedKVCacheKV8 if args.kv == "e4m3" else PagedKVCache
     weights = Qwen3Weights.synthetic(shape, 1234, dev)
     prompt = torch.randint(0, shape.vocab, (P,), generator=torch.Generator().manual_seed(5)).tolist()
     nb = (P + GEN_HEADROOM) // PAGE + 2
     schedules = [(args.prefill_chunk, False)] + ([(PAGE * 32, True)] if args.prefill_aligned else [])
     for chunk, aligned in schedules:
-        kv = PagedKVCache(shape, nb, dev)
-        ver = Qwen3Verifier(weights, kv, max_rows=chunk, max_pos=P + GEN_HEADROOM, device=dev)
+        kv = cache(shape, nb, dev)
+        ver = Qwen3Verifier(weights, kv, max_rows=chunk, max_pos=P + GEN_HEADROOM, device=dev, window=args.window,
+                            sinks=args.sinks)
 
         def once():
             eng = MTPVerifyEngine(ver, num_blocks=nb, max_model_len=P + GEN_HEADROOM,
@@ -932,7 +954,8 @@ def run_prefill(args) -> None:
         ver.op_timing = False
         print(json.dumps({"prefill_tokens": P, "chunk": chunk, "page_aligned": aligned, "ms": round(t * 1e3, 1),
                           "cold_ms": round(cold * 1e3, 1), "tok_s": round(P / t, 1), "first_token": first,
-                          "pages": npages, "op_ms": ops, "model": "Qwen3-8B W4A16 g128 (synthetic weights)"}),
+                          "pages": npages, "op_ms": ops, "model": "Qwen3-8B W4A16 g128 (synthetic weights)",
+                          **kv_config(args)}),
               flush=True)
         del ver, kv
         torch.cuda.empty_cache()
@@ -1194,8 +1217,8 @@ def main():
     ap.add_argument("--seqs", type=int, default=SEQS, help="sequences per GPU (default: the BASELINE config)")
     ap.add_argument("--prompt", type=int, default=PROMPT, help="prompt tokens per sequence")
     ap.add_argument("--kv", default="bf16", choices=["bf16", "e4m3"],
-                    help="KV cache of the bench line: bf16 (the default workload) or 8-bit e4m3 codes with a scale "
-                         "per page and KV head")
+                    help="KV cache of the bench line and of --prefill: bf16 (the default workload) or 8-bit e4m3 codes "
+                         "with a scale per page and KV head")
     ap.add_argument("--window", type=int, default=0, help="with --kv e4m3: sliding attention window (0: none)")
     ap.add_argument("--sinks", type=int, default=0, help="with --window: first tokens that stay visible")
     ap.add_argument("--layers", type=int, default=0, help="decoder layers (0 = all 36); profiling only")
@@ -1215,6 +1238,7 @@ def main():
     ap.add_argument("--prefill-aligned", action="store_true",
                     help="prefill: also time the reference's page-aligned chunk schedule")
     args = ap.parse_args()
+    check_kv_flags(ap, args)
     if args.prefill:
         run_prefill(args)
         return
