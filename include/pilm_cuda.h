@@ -520,8 +520,8 @@ int ekernel_qk_norm_rope_kv_append_kv8_splitk(const ekernel_paged_attn_desc_t *d
  *    row's own (exact for elements down to 2^-28 of the row's largest), keys exactly.  A key's
  *    probability times its page's V scale, p * vs, is rounded to f16 for the product with V: 11 bits
  *    down to 2^-23 of the largest p * vs among the keys that the row sees, steps of 2^-33 of it below
- *    (a page of zero codes counts by its scale like any other).  The output is rounded once, after
- *    the gate.
+ *    (a page of zero codes counts by its scale like any other; a p below 2^-118 may count as 0,
+ *    whatever its vs).  The output is rounded once, after the gate.
  *  - workspace: at least ekernel_paged_attention_kv8_workspace_bytes(desc, window, sinks)
  *    bytes (never 0, for an empty batch neither; 0 means a refused descriptor), 16-byte aligned, its contents undefined before and after.  The library allocates
  *    none of its own, so calls that may overlap on the GPU (other streams, other graphs) need
