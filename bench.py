@@ -215,23 +215,12 @@ def greedy_rollout(eng, n_tokens: int, k: int):
     return drafts
 
 
-def timed_warm(eng, timed, agree=lambda n: n, tries: int = 3):
-    """(timed(), graphs captured in it) of the first run that captures none: verify_step captures a
-    graph the first time that it meets a batch's shape, and a run whose drafts are accepted raggedly
-    meets new ones as it goes.  Each further run starts from the same sequences.  After `tries` runs the
-    last one counts.  agree: the number over all ranks, which repeat together."""
-    run = list(eng.sched.running)
-    base = [(len(s.tokens), len(s.outputs), s.num_computed) for s in run]
-    for i in range(tries):
-        before = len(eng.graphs)
-        out = timed()
-        captured = agree(len(eng.graphs) - before)
-        if not captured or i + 1 == tries:
-            return out, captured
-        for s, (nt, no, nc) in zip(run, base):
-            del s.tokens[nt:]
-            del s.outputs[no:]
-            s.num_computed = nc
+def without_captures(steps: list[dict]) -> tuple[dict, int]:
+    """(mean per step of each figure over the steps that captured no graph, number of those that did).
+    verify_step captures a graph the first time that it meets a batch's shape, which takes longer than the
+    step; drafts accepted raggedly bring new shapes at any time.  All steps count where each one captured."""
+    kept = [s for s in steps if not s["captured"]] or steps
+    return {k: sum(s[k] for s in kept) / len(kept) for k in kept[0]}, sum(bool(s["captured"]) for s in steps)
 
 
 def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
@@ -412,37 +401,32 @@ def run_ours(args, rank: int, world: int, local_rank: int) -> dict | None:
 
         for _ in range(n_warm):
             eng.verify_step(ideal_drafts())
-
-        def timed():
-            torch.cuda.synchronize()
-            if world > 1:
-                dist.barrier()
-            a_rows = a_tokens = a_att = a_acc = 0
-            a0, a1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-            a0.record(stream)
-            for _ in range(e2e_steps):
-                d = ideal_drafts()
-                rows_before = eng.stats["verified_rows"]
-                for r in eng.verify_step(d):
-                    a_tokens += 1 + r.accepted
-                    a_att += len(r.drafts)
-                    a_acc += r.accepted
-                a_rows += eng.stats["verified_rows"] - rows_before
-            a1.record(stream)
-            torch.cuda.synchronize()
-            return a0.elapsed_time(a1) / e2e_steps, a_rows, a_tokens, a_att, a_acc
-
-        (a_ms, a_rows, a_tokens, a_att, a_acc), captured = timed_warm(
-            eng, timed, lambda n: int(reduce_over_ranks([float(n)], [], dev)[0][0]))
-        (a_ms,), (a_rows_all, a_tokens_all) = reduce_over_ranks([a_ms], [float(a_rows), float(a_tokens)], dev)
+        torch.cuda.synchronize()
+        if world > 1:
+            dist.barrier()
+        steps, events = [], [torch.cuda.Event(enable_timing=True) for _ in range(e2e_steps + 1)]
+        events[0].record(stream)
+        for i in range(e2e_steps):
+            d = ideal_drafts()
+            rows_before, graphs_before = eng.stats["verified_rows"], len(eng.graphs)
+            res = eng.verify_step(d)
+            events[i + 1].record(stream)
+            steps.append({"tokens": len(res) + sum(r.accepted for r in res), "att": sum(len(r.drafts) for r in res),
+                          "acc": sum(r.accepted for r in res), "rows": eng.stats["verified_rows"] - rows_before,
+                          "captured": len(eng.graphs) - graphs_before})
+        torch.cuda.synchronize()
+        for i, s in enumerate(steps):
+            s["ms"] = events[i].elapsed_time(events[i + 1])
+        mean, captured = without_captures(steps)
+        (a_ms,), (a_rows, a_tokens) = reduce_over_ranks([mean["ms"]], [mean["rows"], mean["tokens"]], dev)
         eng.graphs = {}
         return {
-            "verified_tok_s": round(a_rows_all / e2e_steps / (a_ms * 1e-3), 2),
-            "accepted_tok_s": round(a_tokens_all / e2e_steps / (a_ms * 1e-3), 2),
+            "verified_tok_s": round(a_rows / (a_ms * 1e-3), 2),
+            "accepted_tok_s": round(a_tokens / (a_ms * 1e-3), 2),
             "ms_per_step": round(a_ms, 4),
             "draft_k": K_DRAFT,
-            "accept_rate": round(a_acc / max(1, a_att), 4),
-            **({"graphs_captured": captured} if captured else {}),
+            "accept_rate": round(mean["acc"] / max(1, mean["att"]), 4),
+            **({"steps_left_out_for_captures": captured} if captured else {}),
             "drafts": "the target model's own greedy continuation (computed untimed beforehand)",
             "call": "pilm_b200.engine.MTPVerifyEngine.verify_step (host drafts -> host accept results)",
         }
