@@ -905,17 +905,15 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
         if (lane == 0) s_ml[warp][0] = sum.m, s_ml[warp][1] = sum.l;
         __syncthreads();
         if (sub) return;
-        for (int w = 1; w < wpi; w += 4) {  // wpi is a power of two
-            float m[4], l[4];
-            float4 o[4];
+        float m[WPB - 1], l[WPB - 1];  // the others' sums
+        float4 o[WPB - 1];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int at = warp + min(w + u, wpi - 1);
-                m[u] = w + u < wpi ? s_ml[at][0] : -INFINITY, l[u] = w + u < wpi ? s_ml[at][1] : 0.f;
-                o[u] = *reinterpret_cast<const float4 *>(&s_o[at][4 * lane]);
-            }
-            sum.add(m, l, o);
+        for (int u = 0; u < WPB - 1; ++u) {
+            const int at = warp + min(u + 1, wpi - 1);
+            m[u] = u + 1 < wpi ? s_ml[at][0] : -INFINITY, l[u] = u + 1 < wpi ? s_ml[at][1] : 0.f;
+            o[u] = *reinterpret_cast<const float4 *>(&s_o[at][4 * lane]);
         }
+        sum.add(m, l, o);
     }
     if (!cut) return;
     const size_t ob = ((size_t)(q0 + j) * p.nh + head) * kHD + 4 * lane;
