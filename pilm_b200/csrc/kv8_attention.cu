@@ -284,7 +284,7 @@ __device__ __forceinline__ int cta_of(int x, int T, int G) {
 // Measured, in a captured graph: 96 verify rows over 32 x 8236 keys, 32 + 8 heads: 93.5 us with the
 // merge, 5.1 TB/s of cache, where the copy of as many bytes takes 74 us and this kernel with its
 // arithmetic left out 89 (sums of pages differ by up to a block of 0.8 us between the CTAs, and the
-// first bytes arrive 5 us after the start).  One row over 131071 keys 54.8 us, 4.9 TB/s; one row over 301
+// first bytes arrive 5 us after the start).  One row over 131071 keys 54.4 us, 4.9 TB/s; one row over 301
 // keys 8.2 us, a chain of loads (lengths and page ids -> pages), two rounds of products and a join.
 // ---------------------------------------------------------------------------------
 constexpr int kTokWarps = 8;      // consumer warps at most
@@ -949,7 +949,8 @@ __global__ void __launch_bounds__(WPB * 32) kv8_attn_merge(const TokParams p, in
 // card's f16 rate: 118); 8192 rows through a 1024-key window with 4 sinks 231 us, 560 TFLOP/s.  A
 // block of both tiles takes 2.0 to 2.4 us, of which the tensor cores work 1.5 (an M = 128, N = 128
 // product takes 88 cycles of the ideal 64) and the exponentials 1.04; a tile's next scores wait for its
-// P to be used, as TMEM is full.  A CTA's first scores come 6 us after its start, its last stores 4 us
+// P to be used: with two tiles TMEM is full (a CTA with one tile takes the same turns, although the
+// other's columns are idle).  A CTA's first scores come 6 us after its start, its last stores 4 us
 // after the last P.
 // Measured and left out: 64-key blocks with two score buffers (349 us: N = 64 products cost nearly what N = 128
 // ones do, twice the hand-overs), 16 softmax warps (348), scores held in registers, and blocks that take over
@@ -1610,7 +1611,8 @@ struct ChunkPlan {
 // however few of their rows are used; the token kernel converts the cache anew for every 16-row tile
 // and reads it anew for every eight.  Measured (us, token against chunk): 32 sequences over 8K keys,
 // 8 KV heads, 32 rows 167 against 239, 40 rows 309 against 240; 24 sequences over 2.5K keys, 2 KV
-// heads, 40 rows 31 against 24; one sequence of 40 rows over 8K keys 14.6 against 15.9.
+// heads, 40 rows 31 against 24; one sequence of 40 rows over 8K keys 14.6 against 15.9, which is what a
+// rule on rows alone costs there.
 constexpr long long kChunkRows = 33;
 
 bool plan_chunks(const ekernel_paged_attn_desc_t *d, size_t window, size_t sinks, ChunkPlan &c) {
