@@ -121,3 +121,26 @@ def test_the_same_call_gives_the_same_bits(q_lens, ctxs, nh, nkv, window):
         ck.paged_attention_verify_kv8(desc, q, *cache, table_of(b), i32(b.cu), i32(b.ctxs), None, out, window=window, workspace=ws)
         want = out if want is None else want
         assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("seqs,rows", [(0, 0), (2, 0), (0, 3)])
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_empty_batches_through_the_wrappers(seqs, rows, max_q):
+    """No rows, no sequences or neither, with the workspace allocated by the call: nothing is written."""
+    d, nh, nkv = dev(), 8, 2
+    cache = ref.random_cache(4, nkv, 1, d)
+    before = [t.clone() for t in cache]
+    desc = ck.attn_desc(num_seqs=seqs, total_q=rows, max_q_len=max_q, n_heads=nh, n_kv_heads=nkv, head_dim=HD, block_size=16,
+                        num_blocks=4, max_blocks_per_seq=4, max_context=64, qkv_stride=(nh + 2 * nkv) * HD, rope_rows=64,
+                        rot_dim=HD, eps=1e-6, add_one=0, output_gate=0)
+    q = torch.zeros((rows, nh * HD), dtype=torch.bfloat16, device=d)
+    out = torch.full_like(q, 7.25)
+    table = torch.zeros((seqs, 4), dtype=torch.int32, device=d)
+    ck.paged_attention_verify_kv8(desc, q, *cache, table, i32([0] * (seqs + 1)), i32([0] * seqs), None, out)
+    if rows == 0:
+        one, angle = torch.ones(HD, dtype=torch.bfloat16, device=d), torch.ones((64, 64), device=d)
+        none = i32([])
+        ck.qk_norm_rope_kv_append_kv8(desc, torch.empty((0, (nh + 2 * nkv) * HD), dtype=torch.bfloat16, device=d), one, one, angle,
+                                      angle, none, none, *cache, q)
+    torch.cuda.synchronize()
+    assert (out == 7.25).all() and all(torch.equal(x, y) for x, y in zip(before, cache))
